@@ -16,7 +16,11 @@ OBJ = os.path.join(HERE, 'build')
 LIB = os.path.join(HERE, 'lib', 'libmmdgan_hip.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function',
-         '-Wno-unused-result']
+         '-Wno-unused-result',
+         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this part now
+         # and then, without an error.  Costs 1.5 % of a CIFAR step (1.758 -> 1.785 ms) and 2 % of a CelebA / ResNet-SN one.  The
+         # host pass does not know the feature and says so.
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _newer(src, deps, out):
@@ -44,8 +48,9 @@ def build(force=False, verbose=True):
         return job, r
     with concurrent.futures.ThreadPoolExecutor(max_workers=8) as ex:
         for (s, o), r in ex.map(cc, jobs):
-            if verbose and (r.returncode != 0 or r.stderr.strip()):
-                sys.stderr.write(r.stderr)
+            err = ''.join(l for l in r.stderr.splitlines(True) if 'packed-fp32-ops' not in l)
+            if verbose and (r.returncode != 0 or err.strip()):
+                sys.stderr.write(err)
             if r.returncode != 0:
                 raise RuntimeError('hipcc failed on %s' % s)
     objs = [os.path.join(OBJ, os.path.basename(s)[:-4] + '.o') for s in srcs]
