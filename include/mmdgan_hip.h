@@ -78,9 +78,10 @@ const char *mmdgan_last_error(void);
  * (200: rounds 1-4 - although mmdgan_bn_bwd gained `beta` and mmdgan_bn_workspace_bytes grew in round 4 without a bump;
  * 500: round 5 - mmdgan_wgrad_defer / mmdgan_wgrad_flush, BN workspace documented as [slots][2][C];
  * 600: round 6 - mmdgan_wino_algo / _algo_weight_bytes / _transform_algo, mmdgan_wino_job.algo, MMDGAN_ACT_FLAG_W_WINOGRAD43;
- * 610: mmdgan_wgrad_algo, the F(4x4,3x3) weight gradient in the default selection).  A caller compares
+ * 610: mmdgan_wgrad_algo, the F(4x4,3x3) weight gradient in the default selection;
+ * 620: mmdgan_gn_*, mmdgan_orthogonalize, mmdgan_muon_update).  A caller compares
  * mmdgan_version() of the library it loaded with the MMDGAN_VERSION it was built against (mmdgan_hip/_lib.py does). */
-#define MMDGAN_VERSION 610
+#define MMDGAN_VERSION 620
 int mmdgan_version(void);
 /* Which kernel a convolution call takes is decided by the geometry and by a handful of process-wide switches (environment
  * variables MMDGAN_*, read once: csrc/tuning.h lists them with their defaults - the defaults are the configuration the
@@ -352,6 +353,28 @@ int mmdgan_bn_fwd_infer(const float *x, long rows, int C, const float *gamma, co
 int mmdgan_bn_bwd(const float *x, const float *y, const float *dy, long rows, int C, const float *gamma,
                   const float *beta, const float *save_mean, const float *save_invstd, int act, float *dx,
                   float *dgamma, float *dbeta, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Group norm with the following activation, NHWC: x [N, HW, C], channels in G groups of C / G (version 620).
+ *   fwd: mean, rstd = 1 / sqrt(var + eps) of each image's group (biased variance over its HW * C / G values),
+ *        y = act((x - mean) * rstd * gamma[c] + beta[c]); writes stats [N][G][2] DOUBLES: mean, rstd.  y may be x.
+ *   bwd: dx, dgamma, dbeta from dy (gradient w.r.t. y), x and the forward call's gamma, beta and stats (y is not read: the
+ *        activation's derivative is decided from x, in 64 bits).  dgamma / dbeta [C] are overwritten; each may be NULL.  dx may be
+ *        dy.  x_batch: how many images x and stats hold (0 = N).  If fewer than N (at least N / 2), the trailing N - x_batch images
+ *        of dy belong to the LAST N - x_batch images of x once more - mmdgan_conv2d_dgrad's dact_batch - and dgamma / dbeta
+ *        are formed from the first x_batch images of dy.
+ * Unlike batch norm the rows stay independent and there are no moving statistics: inference is the forward call.
+ * workspace: mmdgan_gn_workspace_bytes(N, HW, C, G) bytes of device scratch, 16-byte aligned, nothing kept in it between
+ * calls (two calls that may overlap in time need one each).  Sums in a fixed order: equal inputs give equal bits.
+ * 16-byte aligned tensors with C % 4 == 0 get the float4 kernels, others scalar ones.  N <= 65535, HW * C < 2^31.
+ * (The reference has batch norm only, layer_func.py:955-966: 'act_nm': 'gn' is this library's addition.)
+ * ---------------------------------------------------------------------------------------------- */
+size_t mmdgan_gn_workspace_bytes(int N, long HW, int C, int G);      /* 0: not a geometry the entries accept */
+int mmdgan_gn_fwd(const float *x, int N, long HW, int C, int G, const float *gamma, const float *beta, float eps, int act,
+                  float *y, double *stats, void *workspace, void *stream);
+int mmdgan_gn_bwd(const float *x, const float *dy, int N, int x_batch, long HW, int C, int G, const float *gamma,
+                  const float *beta, const double *stats, int act, float *dx, float *dgamma, float *dbeta, void *workspace,
+                  void *stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Spectral normalisation helpers (math_func.py:639-672).  The linear maps themselves are the

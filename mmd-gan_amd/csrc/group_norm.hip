@@ -1,0 +1,586 @@
+// Group normalisation over [N, HW, C] (NHWC), channels in G groups of D = C / G, with the following activation fused.
+//
+//   forward    mean, rstd = 1 / sqrt(var + eps) over the HW * D values of one image's group
+//              z = (x - mean) * rstd * gamma[c] + beta[c],   y = act(z)
+//   backward   dz = dy * act'(z),  xhat = (x - mean) * rstd,  M = HW * D
+//              dbeta[c] = sum dz,  dgamma[c] = sum dz * xhat                        (over images and pixels)
+//              dx = rstd * (gamma * dz - m1 - xhat * m2),  m1 = sum gamma dz / M,  m2 = sum gamma dz xhat / M    (per group)
+//
+// Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.  What the kernels do about it:
+//   gn_resident   one workgroup holds an image's channel slab (whole groups, all pixels) in registers between the sums and
+//                 the apply, so every tensor moves once.  Needs D a power of two and a slab of at most 256 KB (forward) /
+//                 128 KB per tensor (backward).
+//   gn_partial + gn_apply   everything else: pixel chunks' sums to the workspace, then the apply pass reads x (and dy) again.
+// All arithmetic on elements is in 64 bits: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for memory
+// either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
+// cancel cleanly from dx.  The sums are formed in a fixed order, without atomics: equal inputs give equal bits.
+#include "common.h"
+
+namespace mmdgan {
+
+constexpr int kGnMaxThreads = 512;                   // 256 VGPRs per wave: at most half of them hold the slab
+constexpr int kGnFwdRegs = 32, kGnBwdRegs = 16;      // float4 per thread and tensor
+constexpr int kGnGrid = 1024;                        // workgroups of a launch: four per CU
+constexpr int kGnSplitCh = 256;                      // channels of a slab in the two-pass form
+
+struct GnArgs {
+    const float *x, *dy, *gamma, *beta;
+    double *stats;               // [N][G][2]: mean, rstd
+    float *out;                  // y / dx
+    double *part;                // backward: [rows][2][C] partial dbeta, dgamma (null: not wanted)
+    double *gpart;               // two-pass form: [N][G][P][2]
+    int N, x_batch, HW, C, G, D;
+    float below;                 // the activation's slope below zero
+    float eps;
+    // resident: slab width, slabs, images per grid row count
+    int S, slabs, rows;
+    // two-pass: channels per slab, groups per slab, pieces a group is cut into, pixel chunks and pixels per chunk
+    int SB, gps, pieces, chunks, chunk_px;
+};
+
+// The activation by its side below zero: 0 relu, 0.1 lrelu, 1 linear (common.h: act_fwd, the same value for every input, NaN
+// included); tanh is a template argument of the kernels - its code in every unrolled element costs registers the others need.
+template <bool TANH> __device__ __forceinline__ float gn_act(float z, float below) {
+    if (TANH) return tanhf(z);
+    return z > 0.f ? z : below == 0.f ? 0.f : z * below;
+}
+template <bool TANH> __device__ __forceinline__ double gn_slope(double z, float below) {
+    if (TANH) { const double t = (double)tanhf((float)z); return 1.0 - t * t; }
+    return z > 0.0 ? 1.0 : (double)below;
+}
+// A value that the compiler must treat as new: without it the 64-bit conversions and normalised values of the first pass over
+// a thread's elements are kept across the barrier for the second (U * 16 more registers: spills from U = 8 on).
+__device__ __forceinline__ void gn_fresh(float4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+// image of x (and of stats) that output image n reads: the images beyond x_batch take the last ones again
+__device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_batch ? n : n - (a.N - a.x_batch); }
+
+// ---- resident form ----------------------------------------------------------------------------------------------
+// Thread t: float4 column t % CV of the slab, pixels t / CV, t / CV + RT, ...; CV = S / 4 and the thread count are powers of two.
+// red: [row groups][K][CV] doubles, then chan: [2][S] (backward totals of this workgroup), gp / stat: [2][groups' pieces].
+template <int U, bool BWD, bool TANH>
+__global__ __launch_bounds__(kGnMaxThreads) void gn_resident_kernel(GnArgs a) {
+    extern __shared__ double gn_lds[];
+    const int T = blockDim.x, t = threadIdx.x, lane = t & 63;
+    const int S = a.S, CV = S >> 2, RT = T / CV, D = a.D, HW = a.HW;
+    const int col = t & (CV - 1), row0 = t / CV;
+    const int wide = CV < 64 ? 64 : CV, RG = T / wide, rg = t / wide;
+    double *red = gn_lds;                              // backward: [RG][8][CV]; forward: the same layout, 2 * GPT of the 8
+    double *chan = red + RG * 8 * CV;                  // [2][S]
+    double *stat = chan + 2 * S;                       // [2][S]: per group (index = its first item / D)
+    const int slab = blockIdx.x % a.slabs, row = blockIdx.x / a.slabs;
+    const int c0 = slab * S + col * 4, g0 = slab * S / D, gps = S / D;
+    const int DW = D < 64 ? D : 64;                    // adjacent channels that one wave reduces by shuffles
+    float4 gv = *reinterpret_cast<const float4 *>(a.gamma + c0), bv = *reinterpret_cast<const float4 *>(a.beta + c0);
+    const double ga[4] = {gv.x, gv.y, gv.z, gv.w}, be[4] = {bv.x, bv.y, bv.z, bv.w};
+    if (BWD && a.part)
+        for (int i = t; i < 2 * S; i += T) chan[i] = 0.0;
+
+    for (int n = row; n < a.N; n += a.rows) {
+        const int ns = gn_src(a, n);
+        const float *px = a.x + (size_t)ns * HW * a.C + c0;
+        const float *pd = BWD ? a.dy + (size_t)n * HW * a.C + c0 : nullptr;
+        float4 vx[U], vd[BWD ? U : 1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = row0 + u * RT;
+            const bool ok = r < HW;
+            vx[u] = ok ? *reinterpret_cast<const float4 *>(px + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (BWD) vd[u] = ok ? *reinterpret_cast<const float4 *>(pd + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        double mean[4], rstd[4];
+        double s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = 0.0;
+        if (BWD) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double *st = a.stats + 2 * ((size_t)ns * a.G + (c0 + j) / D);
+                mean[j] = st[0]; rstd[j] = st[1];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+            if (!BWD) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { const double v = xv[j]; s[j] += v; s[4 + j] = fma(v, v, s[4 + j]); }
+            } else {
+                float dv[4] = {vd[u].x, vd[u].y, vd[u].z, vd[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {              // (a pixel beyond the image holds dy = 0: it adds nothing)
+                    const double xh = ((double)xv[j] - mean[j]) * rstd[j];
+                    double dz = (double)dv[j] * gn_slope<TANH>(fma(xh, ga[j], be[j]), a.below);
+                    if (TANH) { dv[j] = (float)dz; dz = (double)dv[j]; }      // evaluated once: dz itself, in 32 bits, for the second pass
+                    s[j] += dz;
+                    s[4 + j] = fma(dz, xh, s[4 + j]);
+                }
+                if (TANH) vd[u] = make_float4(dv[0], dv[1], dv[2], dv[3]);
+            }
+        }
+        // lanes of a wave that hold the same column
+        for (int o = 32; o >= CV; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] += __shfl_xor(s[k], o, 64);
+        }
+        if (CV >= 64 || lane < CV) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) red[(rg * 8 + k) * CV + col] = s[k];
+        }
+        __syncthreads();
+        // item = channel of the slab: totals over the row groups, then over the group's channels
+        for (int i = t; i < S; i += T) {
+            double s1 = 0.0, s2 = 0.0;
+            for (int q = 0; q < RG; ++q) {
+                s1 += red[(q * 8 + (i & 3)) * CV + (i >> 2)];
+                s2 += red[(q * 8 + 4 + (i & 3)) * CV + (i >> 2)];
+            }
+            if (BWD) {
+                if (a.part && n < a.x_batch) { chan[i] += s1; chan[S + i] += s2; }
+                const double g = (double)a.gamma[slab * S + i];
+                s1 *= g; s2 *= g;
+            }
+            for (int o = DW >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+            if ((i & (DW - 1)) == 0) { stat[i / DW] = s1; stat[S + i / DW] = s2; }
+        }
+        __syncthreads();
+        const double inv_m = 1.0 / ((double)HW * D);
+        const int per = D / DW;
+        double m1[4], m2[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = (col * 4 + j) / D;
+            double s1 = 0.0, s2 = 0.0;
+            for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
+            m1[j] = s1 * inv_m; m2[j] = s2 * inv_m;
+            if (!BWD) {
+                mean[j] = m1[j];
+                double var = m2[j] - m1[j] * m1[j];
+                if (var < 0.0) var = 0.0;
+                rstd[j] = 1.0 / sqrt(var + (double)a.eps);
+            }
+        }
+        if (!BWD) {
+            for (int g = t; g < gps; g += T) {
+                double s1 = 0.0, s2 = 0.0;
+                for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
+                const double mu = s1 * inv_m;
+                double var = s2 * inv_m - mu * mu;
+                if (var < 0.0) var = 0.0;
+                double *st = a.stats + 2 * ((size_t)n * a.G + g0 + g);
+                st[0] = mu; st[1] = 1.0 / sqrt(var + (double)a.eps);
+            }
+        }
+        float *po = a.out + (size_t)n * HW * a.C + c0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = row0 + u * RT;
+            gn_fresh(vx[u]);
+            if (BWD) gn_fresh(vd[BWD ? u : 0]);
+            const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+            float o[4];
+            if (!BWD) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = gn_act<TANH>((float)fma(((double)xv[j] - mean[j]) * rstd[j], ga[j], be[j]), a.below);
+            } else {
+                const float dv[4] = {vd[u].x, vd[u].y, vd[u].z, vd[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double xh = ((double)xv[j] - mean[j]) * rstd[j];
+                    const double dz = TANH ? (double)dv[j] : (double)dv[j] * gn_slope<false>(fma(xh, ga[j], be[j]), a.below);
+                    o[j] = (float)(rstd[j] * (fma(ga[j], dz, -m1[j]) - xh * m2[j]));
+                }
+            }
+            if (r < HW) *reinterpret_cast<float4 *>(po + (size_t)r * a.C) = make_float4(o[0], o[1], o[2], o[3]);
+        }
+        __syncthreads();                               // red and stat are written again for the next image
+    }
+    if (BWD && a.part) {
+        for (int i = t; i < S; i += T) {               // (the thread that owns item i wrote chan[i])
+            double *p = a.part + (size_t)row * 2 * a.C + slab * S + i;
+            p[0] = chan[i]; p[a.C] = chan[S + i];
+        }
+    }
+}
+
+// ---- two-pass form ----------------------------------------------------------------------------------------------
+// slab: `gps` whole groups (D <= 256) or one piece of 256 channels of a group (D > 256)
+struct GnSlab { int c0, width, g0, groups, piece; };
+__device__ __forceinline__ GnSlab gn_slab(const GnArgs &a, int s) {
+    GnSlab r;
+    if (a.pieces == 1) {
+        r.g0 = s * a.gps;
+        r.groups = a.G - r.g0 < a.gps ? a.G - r.g0 : a.gps;
+        r.c0 = r.g0 * a.D; r.width = r.groups * a.D; r.piece = 0;
+    } else {
+        r.g0 = s / a.pieces; r.piece = s % a.pieces; r.groups = 1;
+        r.c0 = r.g0 * a.D + r.piece * kGnSplitCh;
+        const int left = a.D - r.piece * kGnSplitCh;
+        r.width = left < kGnSplitCh ? left : kGnSplitCh;
+    }
+    return r;
+}
+
+template <int VEC> __device__ __forceinline__ void gn_load(const float *p, float *v) {
+    if (VEC == 4) {
+        const float4 q = *reinterpret_cast<const float4 *>(p);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+        v[0] = *p;
+    }
+}
+
+template <int VEC, bool BWD, bool TANH>
+__global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
+    constexpr int U = 4;
+    __shared__ double red[2][256 * VEC];
+    __shared__ double chan[2][kGnSplitCh];
+    const int t = threadIdx.x;
+    const int chunk = blockIdx.y, n = blockIdx.z, ns = gn_src(a, n);
+    const GnSlab sl = gn_slab(a, blockIdx.x);
+    const int CV = (sl.width + VEC - 1) / VEC, RT = 256 / CV, rl = t / CV, col = t % CV;
+    const int p0 = chunk * a.chunk_px;
+    const int p1 = p0 + a.chunk_px < a.HW ? p0 + a.chunk_px : a.HW;
+    double s1[VEC], s2[VEC], mean[VEC], rstd[VEC], ga[VEC], be[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { s1[j] = 0.0; s2[j] = 0.0; }
+    if (rl < RT) {
+        const int c = sl.c0 + col * VEC;
+        if (BWD) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const double *st = a.stats + 2 * ((size_t)ns * a.G + (c + j) / a.D);
+                mean[j] = st[0]; rstd[j] = st[1]; ga[j] = a.gamma[c + j]; be[j] = a.beta[c + j];
+            }
+        }
+        const float *px = a.x + (size_t)ns * a.HW * a.C + c;
+        const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
+        for (int r = p0 + rl; r < p1; r += RT * U) {
+            float vx[U][VEC], vd[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int rr = r + u * RT;
+                const bool ok = rr < p1;
+                if (ok) gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
+                if (BWD && ok) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
+                if (!ok) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) { vx[u][j] = 0.f; vd[u][j] = 0.f; }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const double v = vx[u][j];
+                    if (!BWD) { s1[j] += v; s2[j] = fma(v, v, s2[j]); }
+                    else {
+                        const double xh = (v - mean[j]) * rstd[j];
+                        const double dz = (double)vd[u][j] * gn_slope<TANH>(fma(xh, ga[j], be[j]), a.below);
+                        s1[j] += dz; s2[j] = fma(dz, xh, s2[j]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            red[0][rl * CV * VEC + col * VEC + j] = s1[j];
+            red[1][rl * CV * VEC + col * VEC + j] = s2[j];
+        }
+    }
+    __syncthreads();
+    for (int i = t; i < sl.width; i += 256) {
+        double u1 = 0.0, u2 = 0.0;
+        for (int q = 0; q < RT; ++q) { u1 += red[0][q * CV * VEC + i]; u2 += red[1][q * CV * VEC + i]; }
+        if (BWD) {
+            if (a.part && n < a.x_batch) {
+                double *p = a.part + ((size_t)n * a.chunks + chunk) * 2 * a.C + sl.c0 + i;
+                p[0] = u1; p[a.C] = u2;
+            }
+            const double g = (double)a.gamma[sl.c0 + i];
+            u1 *= g; u2 *= g;
+        }
+        chan[0][i] = u1; chan[1][i] = u2;
+    }
+    __syncthreads();
+    const int P = a.chunks * a.pieces, p = chunk * a.pieces + sl.piece;
+    const int per = sl.groups == 1 ? sl.width : a.D;   // channels of a group in this slab
+    if (per <= 8) {
+        for (int g = t; g < sl.groups; g += 256) {
+            double u1 = 0.0, u2 = 0.0;
+            for (int q = 0; q < per; ++q) { u1 += chan[0][g * per + q]; u2 += chan[1][g * per + q]; }
+            double *o = a.gpart + (((size_t)n * a.G + sl.g0 + g) * P + p) * 2;
+            o[0] = u1; o[1] = u2;
+        }
+    } else {
+        for (int g = t >> 6; g < sl.groups; g += 4) {
+            double u1 = 0.0, u2 = 0.0;
+            for (int q = t & 63; q < per; q += 64) { u1 += chan[0][g * per + q]; u2 += chan[1][g * per + q]; }
+            u1 = wave_sum(u1); u2 = wave_sum(u2);
+            if ((t & 63) == 0) {
+                double *o = a.gpart + (((size_t)n * a.G + sl.g0 + g) * P + p) * 2;
+                o[0] = u1; o[1] = u2;
+            }
+        }
+    }
+}
+
+template <int VEC, bool BWD, bool TANH>
+__global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
+    constexpr int U = 4;
+    __shared__ double stat[2][kGnSplitCh];             // per group of the slab: mean, rstd / m1, m2
+    const int t = threadIdx.x;
+    const int chunk = blockIdx.y, n = blockIdx.z, ns = gn_src(a, n);
+    const GnSlab sl = gn_slab(a, blockIdx.x);
+    const int CV = (sl.width + VEC - 1) / VEC, RT = 256 / CV, rl = t / CV, col = t % CV;
+    const int p0 = chunk * a.chunk_px;
+    const int p1 = p0 + a.chunk_px < a.HW ? p0 + a.chunk_px : a.HW;
+    const int P = a.chunks * a.pieces;
+    const double inv_m = 1.0 / ((double)a.HW * a.D);
+    auto publish = [&](int g, double u1, double u2) {
+        if (BWD) { stat[0][g] = u1 * inv_m; stat[1][g] = u2 * inv_m; return; }
+        const double mu = u1 * inv_m;
+        double var = u2 * inv_m - mu * mu;
+        if (var < 0.0) var = 0.0;
+        const double is = 1.0 / sqrt(var + (double)a.eps);
+        stat[0][g] = mu; stat[1][g] = is;
+        if (chunk == 0 && sl.piece == 0) {
+            double *st = a.stats + 2 * ((size_t)n * a.G + sl.g0 + g);
+            st[0] = mu; st[1] = is;
+        }
+    };
+    if (P <= 8) {
+        for (int g = t; g < sl.groups; g += 256) {
+            const double *q = a.gpart + ((size_t)n * a.G + sl.g0 + g) * P * 2;
+            double u1 = 0.0, u2 = 0.0;
+            for (int p = 0; p < P; ++p) { u1 += q[2 * p]; u2 += q[2 * p + 1]; }
+            publish(g, u1, u2);
+        }
+    } else {
+        for (int g = t >> 6; g < sl.groups; g += 4) {
+            const double *q = a.gpart + ((size_t)n * a.G + sl.g0 + g) * P * 2;
+            double u1 = 0.0, u2 = 0.0;
+            for (int p = t & 63; p < P; p += 64) { u1 += q[2 * p]; u2 += q[2 * p + 1]; }
+            u1 = wave_sum(u1); u2 = wave_sum(u2);
+            if ((t & 63) == 0) publish(g, u1, u2);
+        }
+    }
+    __syncthreads();
+    if (rl >= RT) return;
+    const int c = sl.c0 + col * VEC;
+    double mean[VEC], rstd[VEC], m1[VEC], m2[VEC], ga[VEC], be[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int g = (c + j) / a.D - sl.g0;
+        ga[j] = a.gamma[c + j]; be[j] = a.beta[c + j];
+        if (BWD) {
+            const double *st = a.stats + 2 * ((size_t)ns * a.G + sl.g0 + g);
+            mean[j] = st[0]; rstd[j] = st[1]; m1[j] = stat[0][g]; m2[j] = stat[1][g];
+        } else {
+            mean[j] = stat[0][g]; rstd[j] = stat[1][g]; m1[j] = 0.0; m2[j] = 0.0;
+        }
+    }
+    const float *px = a.x + (size_t)ns * a.HW * a.C + c;
+    const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
+    float *po = a.out + (size_t)n * a.HW * a.C + c;
+    for (int r = p0 + rl; r < p1; r += RT * U) {
+        float vx[U][VEC], vd[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = r + u * RT;
+            if (rr < p1) {
+                gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
+                if (BWD) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { vx[u][j] = 0.f; vd[u][j] = 0.f; }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = r + u * RT;
+            float o[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const double xh = ((double)vx[u][j] - mean[j]) * rstd[j], z = fma(xh, ga[j], be[j]);
+                if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
+                else o[j] = (float)(rstd[j] * (fma(ga[j], (double)vd[u][j] * gn_slope<TANH>(z, a.below), -m1[j]) - xh * m2[j]));
+            }
+            if (rr < p1) {
+                if (VEC == 4) *reinterpret_cast<float4 *>(po + (size_t)rr * a.C) = make_float4(o[0], o[1 % VEC], o[2 % VEC], o[3 % VEC]);
+                else po[(size_t)rr * a.C] = o[0];
+            }
+        }
+    }
+}
+
+// dbeta[c] / dgamma[c] = sum of the partial rows, in row order per lane
+__global__ __launch_bounds__(256) void gn_param_kernel(const double *part, long rows, int C, float *dgamma, float *dbeta) {
+    __shared__ double red[2][32][9];
+    const int cl = threadIdx.x & 7, rl = threadIdx.x >> 3;
+    const int c = blockIdx.x * 8 + cl;
+    double s1 = 0.0, s2 = 0.0;
+    if (c < C) {
+#pragma unroll 4
+        for (long r = rl; r < rows; r += 32) { s1 += part[r * 2 * C + c]; s2 += part[r * 2 * C + C + c]; }
+    }
+    red[0][rl][cl] = s1; red[1][rl][cl] = s2;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        const int which = threadIdx.x >> 3, ch = blockIdx.x * 8 + cl;
+        double v = 0.0;
+        for (int q = 0; q < 32; ++q) v += red[which][q][cl];
+        float *out = which == 0 ? dbeta : dgamma;
+        if (ch < C && out) out[ch] = (float)v;
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------
+static inline bool gn_pow2(long v) { return v > 0 && (v & (v - 1)) == 0; }
+
+// How a geometry runs; the same for the workspace query and for the call (which may still fall back from the resident form
+// when a pointer is not 16-byte aligned: the workspace covers both).
+struct GnPlan {
+    bool resident;
+    int S, T, U;                 // resident: slab channels, threads, float4 per thread
+    int SB, gps, pieces, slabs, chunks, chunk_px;     // two-pass
+};
+static void gn_plan_resident(long HW, int C, int D, long N, bool bwd, GnPlan &p) {
+    p.resident = false;
+    if ((C & 3) || !gn_pow2(D) || D > kGnSplitCh) return;
+    int top = 4;                                       // widest power-of-two slab that divides C
+    while (top < kGnSplitCh && C % (top * 2) == 0) top *= 2;
+    if (top < D) return;
+    const long cap = (long)kGnMaxThreads * (bwd ? kGnBwdRegs : kGnFwdRegs);      // float4 per tensor
+    int least = D < 4 ? 4 : D;
+    // a slab of 64 channels where there are workgroups enough with it, down to 16 (64 bytes a pixel) where there are not or
+    // where the image needs it
+    int S = top < 64 ? top : 64;
+    if (S < least) S = least;
+    while (S > least && S > 16 && (N * (C / S) < 256 || HW * (S / 4) > cap)) S >>= 1;
+    if (HW * (S / 4) > cap) return;
+    const long total = HW * (S / 4);
+    long T = 64;
+    while (T < S / 4) T *= 2;
+    while (T < kGnMaxThreads && T * 4 < total) T *= 2;
+    long U = 1;
+    while (T * U < total) U *= 2;
+    p.resident = true;
+    p.S = S; p.T = (int)T; p.U = (int)U;
+}
+static void gn_plan_split(long HW, int C, int D, long N, GnPlan &p) {
+    const int G = C / D;
+    if (D <= kGnSplitCh) { p.gps = kGnSplitCh / D < G ? kGnSplitCh / D : G; p.pieces = 1; p.SB = p.gps * D; p.slabs = (G + p.gps - 1) / p.gps; }
+    else { p.gps = 1; p.pieces = (D + kGnSplitCh - 1) / kGnSplitCh; p.SB = kGnSplitCh; p.slabs = G * p.pieces; }
+    // pixel chunks: four workgroups per CU in all, at least 64 pixels each
+    long want = (4L * 256 + N * p.slabs - 1) / (N * p.slabs), most = (HW + 63) / 64;
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    if (want < 1) want = 1;
+    p.chunk_px = (int)((HW + want - 1) / want);
+    p.chunks = (int)((HW + p.chunk_px - 1) / p.chunk_px);
+}
+static long gn_resident_rows(long N, int slabs) {
+    const long rows = kGnGrid / slabs > 1 ? kGnGrid / slabs : 1;
+    return rows < N ? rows : N;
+}
+static size_t gn_bytes(long N, long HW, int C, int G) {
+    GnPlan p;
+    gn_plan_split(HW, C, C / G, N, p);
+    const size_t gpart = (size_t)N * G * p.chunks * p.pieces * 2 * sizeof(double);
+    size_t part = (size_t)N * p.chunks * 2 * C * sizeof(double);
+    return gpart + part + 256;
+}
+
+static bool gn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+template <bool BWD, bool TANH>
+static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st) {
+    const int CV = p.S / 4, wide = CV < 64 ? 64 : CV;
+    const size_t lds = ((size_t)(p.T / wide) * 8 * CV + 4 * (size_t)p.S) * sizeof(double);
+    const dim3 grid((unsigned)(a.rows * a.slabs)), block(p.T);
+    switch (p.U) {
+        case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH>), grid, block, lds, st, a); break;
+        case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH>), grid, block, lds, st, a); break;
+        case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH>), grid, block, lds, st, a); break;
+        case 8: hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH>), grid, block, lds, st, a); break;
+        case 16: hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH>), grid, block, lds, st, a); break;
+        default: hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH>), grid, block, lds, st, a); break;   // forward only (plan)
+    }
+}
+
+template <bool BWD, bool TANH>
+static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipStream_t st, const char *what) {
+    GnPlan p;
+    gn_plan_resident(a.HW, a.C, a.D, a.N, BWD, p);
+    if (p.resident && !(gn_aligned(a.x) && gn_aligned(a.out) && gn_aligned(a.gamma) && gn_aligned(a.beta) && (!BWD || gn_aligned(a.dy))))
+        p.resident = false;
+    long part_rows;
+    const bool params = BWD && (dgamma || dbeta);
+    if (p.resident) {
+        a.S = p.S; a.slabs = a.C / p.S;
+        a.rows = (int)gn_resident_rows(a.N, a.slabs);
+        part_rows = a.rows;
+        a.part = params ? (double *)workspace : nullptr;
+        gn_launch_resident<BWD, TANH>(a, p, st);
+    } else {
+        gn_plan_split(a.HW, a.C, a.D, a.N, p);
+        a.SB = p.SB; a.gps = p.gps; a.pieces = p.pieces; a.slabs = p.slabs; a.chunks = p.chunks; a.chunk_px = p.chunk_px;
+        a.gpart = (double *)workspace;
+        part_rows = (long)a.x_batch * a.chunks;
+        a.part = params ? a.gpart + (size_t)a.N * a.G * a.chunks * a.pieces * 2 : nullptr;
+        const bool vec = !(a.C & 3) && (a.pieces == 1 ? !(a.SB & 3) : !(a.D & 3)) && gn_aligned(a.x) && gn_aligned(a.out) && (!BWD || gn_aligned(a.dy));
+        const dim3 grid(p.slabs, p.chunks, a.N), block(256);
+        if (vec) {
+            hipLaunchKernelGGL((gn_partial_kernel<4, BWD, TANH>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((gn_apply_kernel<4, BWD, TANH>), grid, block, 0, st, a);
+        } else {
+            hipLaunchKernelGGL((gn_partial_kernel<1, BWD, TANH>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((gn_apply_kernel<1, BWD, TANH>), grid, block, 0, st, a);
+        }
+    }
+    if (params) hipLaunchKernelGGL(gn_param_kernel, dim3((a.C + 7) / 8), dim3(256), 0, st, a.part, part_rows, a.C, dgamma, dbeta);
+    return check_launch(what);
+}
+template <bool BWD>
+static int gn_dispatch(GnArgs &a, int act, float *dgamma, float *dbeta, void *workspace, hipStream_t st, const char *what) {
+    if (act == MMDGAN_ACT_TANH) return gn_run<BWD, true>(a, dgamma, dbeta, workspace, st, what);
+    a.below = act == MMDGAN_ACT_RELU ? 0.f : act == MMDGAN_ACT_LRELU ? kLreluAlpha : 1.f;
+    return gn_run<BWD, false>(a, dgamma, dbeta, workspace, st, what);
+}
+}  // namespace mmdgan
+
+using namespace mmdgan;
+
+#define GN_REQUIRE_GEOMETRY(what)                                                                                                    \
+    MMDGAN_REQUIRE(N >= 1 && HW >= 1 && C >= 1 && G >= 1, what ": bad size N=%d HW=%ld C=%d G=%d", N, HW, C, G);                      \
+    MMDGAN_REQUIRE(C % G == 0, what ": %d channels do not divide into %d groups", C, G);                                              \
+    MMDGAN_REQUIRE(N <= 65535 && HW <= 0x7fffffffL / C, what ": image of %ld pixels x %d channels or batch of %d is too large", HW, C, N); \
+    MMDGAN_REQUIRE(act >= MMDGAN_ACT_LINEAR && act <= MMDGAN_ACT_TANH, what ": unknown activation %d", act)
+
+extern "C" size_t mmdgan_gn_workspace_bytes(int N, long HW, int C, int G) {
+    if (N < 1 || HW < 1 || C < 1 || G < 1 || C % G) return 0;
+    return gn_bytes(N, HW, C, G);
+}
+extern "C" int mmdgan_gn_fwd(const float *x, int N, long HW, int C, int G, const float *gamma, const float *beta, float eps, int act,
+                             float *y, double *stats, void *workspace, void *stream) {
+    MMDGAN_REQUIRE(x && gamma && beta && y && stats && workspace, "gn_fwd: null pointer");
+    GN_REQUIRE_GEOMETRY("gn_fwd");
+    MMDGAN_REQUIRE(eps > 0.f, "gn_fwd: eps must be positive");
+    GnArgs a{};
+    a.x = x; a.gamma = gamma; a.beta = beta; a.stats = stats; a.out = y;
+    a.N = a.x_batch = N; a.HW = (int)HW; a.C = C; a.G = G; a.D = C / G; a.eps = eps;
+    return gn_dispatch<false>(a, act, nullptr, nullptr, workspace, (hipStream_t)stream, "gn_fwd");
+}
+extern "C" int mmdgan_gn_bwd(const float *x, const float *dy, int N, int x_batch, long HW, int C, int G, const float *gamma,
+                             const float *beta, const double *stats, int act, float *dx, float *dgamma, float *dbeta,
+                             void *workspace, void *stream) {
+    MMDGAN_REQUIRE(x && dy && gamma && beta && stats && dx && workspace, "gn_bwd: null pointer");
+    GN_REQUIRE_GEOMETRY("gn_bwd");
+    if (x_batch == 0) x_batch = N;
+    MMDGAN_REQUIRE(x_batch >= 1 && x_batch <= N && N - x_batch <= x_batch, "gn_bwd: x_batch %d for %d images", x_batch, N);
+    MMDGAN_REQUIRE(dx != x || x_batch == N, "gn_bwd: dx must not be x when images of x are read twice");
+    GnArgs a{};
+    a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.stats = const_cast<double *>(stats); a.out = dx;
+    a.N = N; a.x_batch = x_batch; a.HW = (int)HW; a.C = C; a.G = G; a.D = C / G;
+    return gn_dispatch<true>(a, act, dgamma, dbeta, workspace, (hipStream_t)stream, "gn_bwd");
+}

@@ -73,6 +73,9 @@ SIGNATURES = {
     'mmdgan_conv2d_dgrad_stats': (_I, [_G, _P, _P, _P, _P, _I, _P, _P, _P]),
     'mmdgan_bn_fwd_infer': (_I, [_P, _L, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
     'mmdgan_bn_bwd': (_I, [_P, _P, _P, _L, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P]),
+    'mmdgan_gn_workspace_bytes': (ctypes.c_size_t, [_I, _L, _I, _I]),
+    'mmdgan_gn_fwd': (_I, [_P, _I, _L, _I, _I, _P, _P, _F, _I, _P, _P, _P, _P]),
+    'mmdgan_gn_bwd': (_I, [_P, _P, _I, _I, _L, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P]),
     'mmdgan_sn_norm': (_I, [_P, _L, _P, _P, _P]),
     'mmdgan_sn_norm_scale': (_I, [_P, _L, _F, _P, _P, _P, _P]),
     'mmdgan_sn_scale': (_I, [_P, _F, _P, _P]),
@@ -103,7 +106,7 @@ SIGNATURES = {
     'mmdgan_u8_records_to_nhwc': (_I, [_P, _I, _P, _I, _I, _I, _I, _P]),
 }
 
-ABI_VERSION = 610           # include/mmdgan_hip.h: MMDGAN_VERSION this binding was written against
+ABI_VERSION = 620           # include/mmdgan_hip.h: MMDGAN_VERSION this binding was written against
 
 _lib = None
 

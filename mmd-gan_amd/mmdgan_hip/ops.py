@@ -474,6 +474,75 @@ def bn_bwd(x2d, y2d, dy2d, gamma, save_mean, save_invstd, act='linear', dgamma=N
 
 
 # ------------------------------------------------------------------------------------------------
+def group_norm_workspace(N, HW, C, groups, device):
+    """the scratch of group_norm_fwd / group_norm_bwd for x [N, ..., C] with HW pixels per image (mmdgan_gn_workspace_bytes);
+    calls that may overlap in time - two streams, a graph replayed beside eager work - need one each"""
+    n = _lib.load().mmdgan_gn_workspace_bytes(int(N), int(HW), int(C), int(groups))
+    if n == 0:
+        raise ValueError('group_norm: {} channels in {} groups, {} pixels, {} images'.format(C, groups, HW, N))
+    return torch.empty(n, device=device, dtype=torch.uint8)
+
+
+def _gn_geometry(x, gamma, beta, groups):
+    assert x.dim() >= 2, 'group_norm: x is [N, ..., C], channels last'
+    N, C = x.shape[0], x.shape[-1]
+    assert gamma.numel() == C and beta.numel() == C, 'group_norm: gamma and beta have one entry per channel'
+    HW = 1
+    for s in x.shape[1:-1]:
+        HW *= s
+    return N, HW, C, int(groups)
+
+
+def _p64(t, shape):
+    assert t.is_cuda and t.dtype == torch.float64 and t.is_contiguous() and tuple(t.shape) == tuple(shape), \
+        'expected contiguous fp64 CUDA statistics of shape {}'.format(tuple(shape))
+    return t.data_ptr()
+
+
+def _gn_ws(workspace, N, HW, C, G, device):
+    need = _lib.load().mmdgan_gn_workspace_bytes(N, HW, C, G)
+    if workspace is None:
+        return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
+    assert workspace.is_cuda and workspace.numel() * workspace.element_size() >= need, \
+        'group_norm: the workspace holds {} bytes, {} are needed'.format(workspace.numel() * workspace.element_size(), need)
+    return workspace
+
+
+def group_norm_fwd(x, gamma, beta, groups, act='linear', eps=1e-5, out=None, stats=None, workspace=None):
+    """x [N, ..., C] (NHWC, [N, C], ...): y = act(group_norm(x) * gamma + beta) over `groups` groups of C / groups channels
+    and all pixels of each image (mmdgan_gn_fwd).  Returns (y, stats): stats [N, groups, 2] float64 = mean, 1 / sqrt(var + eps), what
+    group_norm_bwd takes.  out may be x.  Training and inference are the same call."""
+    lib = require_device()
+    N, HW, C, G = _gn_geometry(x, gamma, beta, groups)
+    y = out if out is not None else torch.empty_like(x)
+    assert y.shape == x.shape
+    st = stats if stats is not None else torch.empty((N, max(G, 0), 2), device=x.device, dtype=torch.float64)
+    check(lib.mmdgan_gn_fwd(_p(x), N, HW, C, G, _p(gamma), _p(beta), float(eps), act_id(act), _p(y), _p64(st, (N, G, 2)),
+                            _gn_ws(workspace, N, HW, C, G, x.device).data_ptr(), _stream()), 'group_norm_fwd')
+    return y, st
+
+
+def group_norm_bwd(x, dy, gamma, beta, stats, act='linear', out=None, dgamma=None, dbeta=None, workspace=None, param_grads=True):
+    """gradients of group_norm_fwd from dy (w.r.t. y) and the forward call's x, gamma, beta, stats: (dx, dgamma, dbeta), the last
+    two None with param_grads=False.  dy may hold more images than x (at most twice as many): the extra ones belong to x's
+    LAST images once more, as dact_batch of conv2d_dgrad, and add nothing to dgamma / dbeta.  out may be dy."""
+    lib = require_device()
+    xb, HW, C, G = _gn_geometry(x, gamma, beta, stats.shape[1])
+    N = dy.shape[0]
+    assert tuple(dy.shape[1:]) == tuple(x.shape[1:])
+    dx = out if out is not None else torch.empty_like(dy)
+    assert dx.shape == dy.shape
+    if param_grads:
+        dgamma = dgamma if dgamma is not None else torch.empty_like(gamma)
+        dbeta = dbeta if dbeta is not None else torch.empty_like(beta)
+        assert dgamma.numel() == C and dbeta.numel() == C
+    else:
+        dgamma = dbeta = None
+    check(lib.mmdgan_gn_bwd(_p(x), _p(dy), N, xb, HW, C, G, _p(gamma), _p(beta), _p64(stats, (xb, G, 2)), act_id(act), _p(dx),
+                            _p(dgamma), _p(dbeta), _gn_ws(workspace, N, HW, C, G, x.device).data_ptr(), _stream()), 'group_norm_bwd')
+    return dx, dgamma, dbeta
+
+
 def sn_norm(v, normalise=True, out_norm=None, out_v=None):
     lib = require_device()
     norm = out_norm if out_norm is not None else torch.empty(1, device=v.device, dtype=torch.float32)
