@@ -514,6 +514,39 @@ typedef struct {
 int mmdgan_adam_prepare_multi(const mmdgan_adam_prepare_job *jobs, int n, void *stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Orthogonalised updates of matrices (version 620; csrc/muon.hip).  U [rows, cols] row-major (a conv kernel [R,R,C,K] is its
+ * [R*R*C, K] view, a dense kernel itself):
+ *     X0 = U / ||U||_F (0 if U is 0),   X <- a X + b (X X^T) X + c (X X^T)^2 X   `steps` times,  (a, b, c) = (3.4445, -4.7750, 2.0315)
+ * which takes U's singular values to about 1 and keeps its singular vectors: O = the last X.
+ *   orthogonalize  out = O of U = grad                      (param, momentum*, dsigma.. are not read); out may be grad
+ *   muon_update    g = grad_scale * grad, or with apply_fixup and dsigma grad_scale * (scale[0] * grad - (scale[0] / sigma[0]) * dot[0] * dsigma)
+ *                  (the fix-up of mmdgan_adam_segments);  momentum_out = mu * momentum + g;
+ *                  U = nesterov ? g + mu * momentum_out : momentum_out;
+ *                  out = (1 - lr * weight_decay) * param - lr * 0.2 * sqrt(max(rows, cols)) * O
+ *                  - the factor gives every matrix an update of root mean square 0.2 lr, an Adam step's size, so that one learning
+ *                  rate serves a net whose vectors stay with Adam.  out may be param, momentum_out may be momentum.
+ * Results are as near to the exact ones as 32-bit products on X give, for ill-conditioned and rank-deficient U too; sums in a fixed
+ * order: equal inputs give equal bits (replicas of a data-parallel job stay identical).  All matrices of a call run
+ * together, phase by phase, 16 at a time (about 20 launches at five steps).  jobs: HOST array, read during the call.
+ * Shorter side <= 8192, longer <= 2^22, rows * cols < 2^31; 1 <= steps <= 16.
+ * workspace: mmdgan_muon_workspace_bytes(jobs, n, steps) bytes (rows, cols of the jobs are read), 16-byte aligned, nothing kept in
+ * it between calls (calls that may overlap in time need one each).  (The reference has 'sgd', 'momentum', 'adam', 'rmsprop',
+ * my_sngan.py:52; this update is the library's addition.)
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct mmdgan_muon_job {
+    const float *grad;
+    float *out;
+    const float *param, *momentum;
+    float *momentum_out;
+    const float *dsigma, *dot, *sigma, *scale;
+    int rows, cols;
+} mmdgan_muon_job;
+size_t mmdgan_muon_workspace_bytes(const mmdgan_muon_job *jobs, int n_jobs, int steps);     /* 0: sizes the entries refuse */
+int mmdgan_orthogonalize(const mmdgan_muon_job *jobs, int n_jobs, int steps, void *workspace, void *stream);
+int mmdgan_muon_update(const mmdgan_muon_job *jobs, int n_jobs, float lr, float momentum, int nesterov, float weight_decay,
+                       float grad_scale, int apply_fixup, int steps, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Elementwise pieces of the residual blocks (layer_func.py:1687-1842), NHWC fp32.
  *   resample_down: y[n,p,q,:] (+)= scale * sum of the factor x factor window of x [N, P*factor, Q*factor, C].
  *                  scale = 1/factor^2 is ImageScaling 'avg' (:1155-1159); scale = 1 is the gradient of 'unpool'.

@@ -842,6 +842,102 @@ def adam_prepare_multi(jobs, beta1=0.5, beta2=0.999):
         arena.prepared = True
 
 
+class MuonJob(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('grad', 'out', 'param', 'momentum', 'momentum_out', 'dsigma', 'dot', 'sigma', 'scale')] + \
+               [('rows', ctypes.c_int), ('cols', ctypes.c_int)]
+
+
+def _matrix_shape(t):
+    """a parameter as a matrix: a conv kernel [R,R,C,K] is [R*R*C, K], a dense kernel itself"""
+    if t.dim() < 2:
+        raise ValueError('a tensor of shape {} is no matrix: vectors stay with Adam'.format(tuple(t.shape)))
+    return t.numel() // max(t.shape[-1], 1), t.shape[-1]
+
+
+def _muon_jobs(tensors):
+    jobs = (MuonJob * len(tensors))()
+    for j, t in zip(jobs, tensors):
+        j.rows, j.cols = _matrix_shape(t)
+    return jobs
+
+
+def _muon_ws(jobs, steps, device, workspace=None):
+    need = _lib.load().mmdgan_muon_workspace_bytes(ctypes.cast(jobs, ctypes.c_void_p), len(jobs), int(steps))
+    if need == 0:
+        raise ValueError('orthogonalised updates: {} matrices ({}), {} steps'.format(
+            len(jobs), ', '.join('%dx%d' % (j.rows, j.cols) for j in jobs), steps))
+    if workspace is None:
+        return torch.empty(need, device=device, dtype=torch.uint8)
+    assert workspace.is_cuda and workspace.numel() * workspace.element_size() >= need, \
+        'the workspace holds {} bytes, {} are needed'.format(workspace.numel() * workspace.element_size(), need)
+    return workspace
+
+
+def orthogonalize_workspace(mats, steps=5):
+    """the scratch of orthogonalize(mats, steps) (mmdgan_muon_workspace_bytes); calls that may overlap in time need one each"""
+    mats = [mats] if torch.is_tensor(mats) else list(mats)
+    return _muon_ws(_muon_jobs(mats), steps, mats[0].device)
+
+
+def orthogonalize(mats, steps=5, out=None, workspace=None):
+    """O for every matrix of a list (or for one tensor): singular values taken to about 1 by `steps` iterates of a quintic, singular
+    vectors kept (mmdgan_orthogonalize).  A tensor of more than two dimensions is its [prod(shape[:-1]), shape[-1]] view.
+    Returns tensors of the same shapes; out may be the inputs."""
+    lib = require_device()
+    single = torch.is_tensor(mats)
+    mats = [mats] if single else list(mats)
+    if not mats:
+        return []
+    outs = ([out] if single else list(out)) if out is not None else [torch.empty_like(t) for t in mats]
+    assert len(outs) == len(mats) and all(o.shape == t.shape for o, t in zip(outs, mats))
+    jobs = _muon_jobs(mats)
+    for j, t, o in zip(jobs, mats, outs):
+        j.grad, j.out = _p(t), _p(o)
+    ws = _muon_ws(jobs, steps, mats[0].device, workspace)
+    check(lib.mmdgan_orthogonalize(ctypes.cast(jobs, ctypes.c_void_p), len(jobs), int(steps), ws.data_ptr(), _stream()),
+          'orthogonalize')
+    return outs[0] if single else outs
+
+
+class MuonGroup:
+    """mmdgan_muon_update over a list of matrix parameters: momentum, orthogonalisation of the momentum matrix, weight decay and
+    the step, all matrices together.  Vectors (biases, norms' gamma / beta) stay with AdamGroup / AdamArena.
+    fixups: per parameter None or dict(dsigma=, dot=, sigma=, scale=) of device tensors, the spectral-norm fix-up applied as the
+    gradient is read (as AdamArena's segments).  out_params / out_momenta: where the results go (default: in place)."""
+
+    fold_fixup = True        # False: the caller applied sn_wgrad_fixup itself (data-parallel replicas, before their all-reduce)
+
+    def __init__(self, params, grads, momenta, fixups=None, out_params=None, out_momenta=None):
+        params, grads, momenta = list(params), list(grads), list(momenta)
+        fixups = list(fixups) if fixups is not None else [None] * len(params)
+        out_params = list(out_params) if out_params is not None else params
+        out_momenta = list(out_momenta) if out_momenta is not None else momenta
+        assert len(params) == len(grads) == len(momenta) == len(fixups) == len(out_params) == len(out_momenta) and params
+        self.keep = (params, grads, momenta, fixups, out_params, out_momenta)
+        self._jobs = _muon_jobs(params)
+        for j, p, g, m, f, po, mo in zip(self._jobs, *self.keep):
+            assert p.shape == g.shape == m.shape == po.shape == mo.shape
+            j.param, j.grad, j.momentum, j.out, j.momentum_out = _p(p), _p(g), _p(m), _p(po), _p(mo)
+            if f is not None:
+                assert f['dsigma'].numel() == p.numel()
+                j.dsigma, j.dot, j.sigma, j.scale = (_p(f[k]) for k in ('dsigma', 'dot', 'sigma', 'scale'))
+        self._ws = {}
+
+    def step(self, lr, momentum=0.95, nesterov=True, weight_decay=0.0, grad_scale=1.0, steps=5, workspace=None):
+        """one update on the current stream.  The group keeps one workspace: updates of one group that may overlap in time
+        (two graphs replayed together) need a `workspace` each."""
+        lib = require_device()
+        if workspace is None:
+            workspace = self._ws.get(steps)
+            if workspace is None:
+                workspace = self._ws[steps] = _muon_ws(self._jobs, steps, self.keep[0][0].device)
+        else:
+            _muon_ws(self._jobs, steps, None, workspace)
+        check(lib.mmdgan_muon_update(ctypes.cast(self._jobs, ctypes.c_void_p), len(self._jobs), float(lr), float(momentum), int(bool(nesterov)),
+                                     float(weight_decay), float(grad_scale), int(self.fold_fixup), int(steps),
+                                     workspace.data_ptr(), _stream()), 'muon_update')
+
+
 def nchw_to_nhwc(x):
     lib = require_device()
     N, C, H, W = x.shape
