@@ -14,10 +14,15 @@
 // 2^-25 / s absolute where lo underflows.  Products are hi hi + hi lo + lo hi in fp32 accumulators (lo lo is 2^-22 of the
 // result): as good as fp32 operands at 16/3 of the fp32 matrix rate.
 //
-// Layout ("packed"): row r of an [R, K] operand is K / 32 groups of 128 bytes, 32 hi halves then 32 lo halves: a 128-byte line
-// per row and 32-wide reduction step, and the MFMA operand of a lane (8 halves) is one 16-byte piece of it.  All sides are
-// padded to 128 with zeros, so the products have no edges.
+// Layout ("packed"): an [R, K] operand is cut into 32 x 16 blocks, row blocks outermost; a block is 2 KB: the 64 lanes' 16-byte
+// MFMA operands of the hi parts in lane order (lane = row % 32 + 32 * (k / 8 % 2), 8 halves along k), then those of the lo parts.
+// Every operand load of a wave is one contiguous kilobyte, from L2 or from LDS, without bank conflicts or swizzles.  All sides are
+// padded to 128 with zeros, so the products have no edges.  Row blocks lie 4 KB further apart than their blocks fill: with m a
+// power of two all workgroups of a product, at the same reduction step, would otherwise read addresses that are equal modulo
+// 128 KB, from the same few memory channels.
 #include "common.h"
+
+#include <algorithm>
 
 namespace mmdgan {
 
@@ -33,93 +38,104 @@ constexpr int kMuChain = 3;                  // steps between two true Gram matr
 constexpr float kMuA = 3.4445f, kMuB = -4.7750f, kMuC = 2.0315f;
 constexpr float kScaleX = 4096.f, kScaleA = 4096.f, kScaleQ = 8192.f, kScaleP = 1024.f;
 
-// offset (in halves) of element (r, k)'s hi part in a packed operand with `ld` = 2 * K halves per row; lo is 32 further
-__host__ __device__ __forceinline__ size_t mu_off(size_t r, int k, int ld) { return r * ld + (size_t)(k >> 5) * 64 + (k & 31); }
+// halves from one row block to the next, of `kb` = K / 16 blocks
+__host__ __device__ __forceinline__ size_t mu_strip(int kb) { return (size_t)kb * 1024 + 2048; }
+// offset (in halves) of element (r, k)'s hi part; lo is 512 further
+__device__ __forceinline__ size_t mu_off(int r, int k, int kb) {
+    return (r >> 5) * mu_strip(kb) + (size_t)(k >> 4) * 1024 + ((r & 31) + ((k >> 3) & 1) * 32) * 8 + (k & 7);
+}
 
 __device__ __forceinline__ void mu_split(float v, f16 &hi, f16 &lo) {
     hi = (f16)v;
     lo = (f16)(v - (float)hi);
 }
+// eight values along k, the first at a multiple of 8, as one piece each of hi and lo
+__device__ __forceinline__ void mu_put8(f16 *o, size_t at, const float (&v)[8]) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { f16 h, l; mu_split(v[i], h, l); hi[i] = h; lo[i] = l; }
+    *reinterpret_cast<f16x8 *>(o + at) = hi;
+    *reinterpret_cast<f16x8 *>(o + at + 512) = lo;
+}
 
 // ---- the product of one tile -------------------------------------------------------------------------------------
-// C[i, j] = sum_k A[i, k] B[j, k] for a (64 TB) x (64 TB) tile, four waves as 2 x 2, each (32 TB) x (32 TB).  Per 32-wide step the
-// workgroup stages 64 TB rows of each operand (128 bytes a row) in LDS, double buffered; 16-byte piece c of row r lies at
-// piece c ^ (r & 7), which spreads the 8 rows that a ds_read_b128 serves per cycle over all banks.
-template <int TB> struct MuTile {
-    static constexpr int kRows = 64 * TB;
-    static constexpr int kStage = 2 * kRows * 128;           // bytes
-    static constexpr int kLds = 2 * kStage;
-};
-template <int TB>
-__device__ __forceinline__ void mu_tile(const f16 *A, int lda, const f16 *B, int ldb, int steps, char *lds, f32x16 (&acc)[TB][TB]) {
-    constexpr int R = MuTile<TB>::kRows, L = 2 * TB;         // 16-byte pieces per thread and operand: R * 8 / 256
+// C[i, j] = sum_k A[i, k] B[j, k] for a 128 x 128 tile, four waves as 2 x 2 of 64 x 64.  Per 32-wide step the workgroup stages four row
+// blocks of each operand (4 KB each, contiguous in memory) in LDS, double buffered.  a / b: the first block of the tile's first row
+// block; sa / sb: halves from one row block to the next.
+constexpr int kMuStage = 8 * 4096;                           // bytes of a stage: four row blocks of a, four of b
+__device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, size_t sb, int steps, char *lds, f32x16 (&acc)[2][2]) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const int pr = t >> 3, pc = t & 7;                       // this thread's piece of rows pr, pr + 32, ...
-    mu_u32x4 ra[L], rb[L];
-    auto fetch = [&](int s) {
+    struct Set { mu_u32x4 a[4], b[4]; } r0, r1;
+    auto fetch = [&](int s, Set &x) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            ra[i] = *reinterpret_cast<const mu_u32x4 *>(A + (size_t)(pr + 32 * i) * lda + s * 64 + pc * 8);
-            rb[i] = *reinterpret_cast<const mu_u32x4 *>(B + (size_t)(pr + 32 * i) * ldb + s * 64 + pc * 8);
+        for (int i = 0; i < 4; ++i) {
+            x.a[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
+            x.b[i] = *reinterpret_cast<const mu_u32x4 *>(b + i * sb + (size_t)s * 2048 + t * 8);
         }
     };
-    auto store = [&](char *buf) {
+    auto store = [&](char *buf, const Set &x) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int r = pr + 32 * i;
-            *reinterpret_cast<mu_u32x4 *>(buf + r * 128 + ((pc ^ (r & 7)) << 4)) = ra[i];
-            *reinterpret_cast<mu_u32x4 *>(buf + (R + r) * 128 + ((pc ^ (r & 7)) << 4)) = rb[i];
+        for (int i = 0; i < 4; ++i) {
+            *reinterpret_cast<mu_u32x4 *>(buf + i * 4096 + t * 16) = x.a[i];
+            *reinterpret_cast<mu_u32x4 *>(buf + (4 + i) * 4096 + t * 16) = x.b[i];
         }
     };
-    f32x16 low[TB][TB];                                      // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
+    f32x16 low[2][2];                                        // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
 #pragma unroll
-    for (int i = 0; i < TB; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < TB; ++j) { acc[i][j] = f32x16{}; low[i][j] = f32x16{}; }
-    const int ar = (w >> 1) * 32 * TB + (lane & 31), br = R + (w & 1) * 32 * TB + (lane & 31), half = lane >> 5;
-    fetch(0);
-    store(lds);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        const char *buf = lds + (s & 1) * MuTile<TB>::kStage;
-        if (s + 1 < steps) fetch(s + 1);
+        for (int j = 0; j < 2; ++j) { acc[i][j] = f32x16{}; low[i][j] = f32x16{}; }
+    const int ar = (w >> 1) * 2 * 4096 + lane * 16, br = (4 + (w & 1) * 2) * 4096 + lane * 16;
+    auto multiply = [&](const char *buf) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            f16x8 ah[TB], al[TB], bh[TB], bl[TB];
+            f16x8 ah[2], al[2], bh[2], bl[2];
 #pragma unroll
-            for (int i = 0; i < TB; ++i) {
-                const int r = ar + 32 * i, q = br + 32 * i, c = ks * 2 + half;
-                ah[i] = *reinterpret_cast<const f16x8 *>(buf + r * 128 + ((c ^ (r & 7)) << 4));
-                al[i] = *reinterpret_cast<const f16x8 *>(buf + r * 128 + (((c + 4) ^ (r & 7)) << 4));
-                bh[i] = *reinterpret_cast<const f16x8 *>(buf + q * 128 + ((c ^ (q & 7)) << 4));
-                bl[i] = *reinterpret_cast<const f16x8 *>(buf + q * 128 + (((c + 4) ^ (q & 7)) << 4));
+            for (int i = 0; i < 2; ++i) {
+                ah[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048);
+                al[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048 + 1024);
+                bh[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048);
+                bl[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048 + 1024);
             }
 #pragma unroll
-            for (int i = 0; i < TB; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < TB; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
                     low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
                     low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
                 }
         }
-        if (s + 1 < steps) store(lds + ((s + 1) & 1) * MuTile<TB>::kStage);
-        __syncthreads();
+    };
+    // loads run two stages ahead of the products (one stage is 768 MFMA cycles, a miss takes longer); the barriers publish LDS
+    // only and leave them in flight.  `steps` is even.
+    fetch(0, r0);
+    fetch(1, r1);
+    store(lds, r0);
+    lds_barrier();
+    for (int s = 0; s < steps; s += 2) {
+        const bool more = s + 2 < steps;
+        if (more) fetch(s + 2, r0);
+        multiply(lds);
+        store(lds + kMuStage, r1);
+        lds_barrier();
+        if (more) fetch(s + 3, r1);
+        multiply(lds + kMuStage);
+        if (more) store(lds, r0);
+        lds_barrier();
     }
 #pragma unroll
-    for (int i = 0; i < TB; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < TB; ++j) acc[i][j] += low[i][j];
+        for (int j = 0; j < 2; ++j) acc[i][j] += low[i][j];
 }
-// row / column within the tile of accumulator element e of block (bi, bj): C layout of the 32x32 MFMA
-template <int TB> __device__ __forceinline__ int mu_row(int bi, int e) {
-    const int t = threadIdx.x;
-    return ((t >> 7) & 1) * 32 * TB + 32 * bi + (e >> 2) * 8 + ((t & 63) >> 5) * 4 + (e & 3);
-}
-template <int TB> __device__ __forceinline__ int mu_col(int bj) {
-    const int t = threadIdx.x;
-    return ((t >> 6) & 1) * 32 * TB + 32 * bj + (t & 31);
-}
+// C layout of the 32x32 MFMA: lane l, element e hold column l % 32, row 8 (e / 4) + 4 (l / 32) + e % 4
+__device__ __forceinline__ int mu_row(int e) { return (e >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (e & 3); }
+__device__ __forceinline__ int mu_col() { return threadIdx.x & 31; }
+
+// A wave's 64 x 64 result in 16 KB of LDS, eight-column groups of row r at group ^ (r & 7): rows are then read 16 bytes a lane by
+// 32 lanes in 32 rows without bank conflicts, columns by neighbouring lanes.
+__device__ __forceinline__ int mu_lds(int r, int c) { return r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7); }
 
 // lower-triangle tile number -> (ti, tj), ti >= tj
 __device__ __forceinline__ void mu_tri(int t, int &ti, int &tj) {
@@ -130,6 +146,25 @@ __device__ __forceinline__ void mu_tri(int t, int &ti, int &tj) {
     tj = t - r * (r + 1) / 2;
 }
 
+// Work item of a workgroup that is number b of its matrix, of n items on n rounded up to 8 workgroups: the eight XCDs take
+// workgroups in turn and each has an L2 of its own - XCD x gets the x-th eighth of the matrix's items, neighbours, which share
+// operands.  (An eighth of every matrix, not of the launch: the matrices' items differ in cost.)  -1: none.
+__device__ __forceinline__ int mu_item(unsigned b, unsigned n) {
+    const unsigned x = b & 7, per = n >> 3, rest = n & 7, i = b >> 3;
+    return i < per + (x < rest ? 1u : 0u) ? (int)(x * per + (x < rest ? x : rest) + i) : -1;
+}
+
+// Which matrix of a launch a workgroup belongs to: `first` holds the matrices' first workgroups (entries beyond the last: none
+// reaches them).  Kept apart from the jobs, in two cache lines at most: a search through the jobs themselves waited for one
+// kernel-argument line after the other.
+template <int N> struct MuFirst { unsigned first[N]; };
+template <int N> __device__ __forceinline__ int mu_which(const MuFirst<N> &f, unsigned b) {
+    int q = 0;
+#pragma unroll
+    for (int i = 1; i < N; ++i) q += b >= f.first[i] ? 1 : 0;
+    return q;
+}
+
 // ---- momentum and norm -------------------------------------------------------------------------------------------
 struct MuPrep {
     const float *grad, *mom;         // mom null: U = grad
@@ -137,35 +172,74 @@ struct MuPrep {
     const float *dsigma, *dot, *sigma, *scale;
     double *part;                    // [blocks]
     long n;
-    unsigned first_block;
+    int vec;
+    unsigned blocks;
 };
-struct MuPrepTable { MuPrep j[kMuGroup]; int n; float momentum, grad_scale; int nesterov; };
+struct MuPrepTable { MuFirst<kMuGroup> f; MuPrep j[kMuGroup]; float momentum, grad_scale; int nesterov; };
 constexpr int kMuPrepPer = 4096;     // elements per workgroup and round
-constexpr int kMuPrepMax = 256;      // workgroups per matrix
+constexpr int kMuPrepMax = 1024;     // workgroups per matrix
 
+__device__ __forceinline__ double mu_prep_one(const MuPrep &p, const MuPrepTable &t, long i, float g, float c0, float c1, float ds, float mom) {
+    g *= c0;
+    if (p.dsigma) g -= c1 * ds;
+    float u = g;
+    if (p.mom) {
+        const float m = __builtin_fmaf(t.momentum, mom, g);
+        p.mom_out[i] = m;
+        u = t.nesterov ? __builtin_fmaf(t.momentum, m, g) : m;
+        if (p.u) p.u[i] = u;
+    }
+    return (double)u * (double)u;
+}
 // U = g (+ momentum), its sum of squares by workgroup.  g = grad_scale * grad, or of a spectrally normalised kernel
-// grad_scale * (scale * grad - (scale / sigma) <grad, W> dsigma/dW)  (Adam's read, elementwise.hip)
+// grad_scale * (scale * grad - (scale / sigma) <grad, W> dsigma/dW)  (Adam's read, elementwise.hip).  HBM-bound.
 __global__ __launch_bounds__(256) void mu_prep_kernel(MuPrepTable t) {
     __shared__ double red[4];
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_block) ++q;
+    const int q = mu_which(t.f, blockIdx.x);
     const MuPrep &p = t.j[q];
-    const unsigned nb = (q + 1 < t.n ? t.j[q + 1].first_block : gridDim.x) - p.first_block, b = blockIdx.x - p.first_block;
+    const unsigned nb = p.blocks, b = blockIdx.x - t.f.first[q];
     float c0 = t.grad_scale, c1 = 0.f;
     if (p.dsigma) { c0 = t.grad_scale * p.scale[0]; c1 = t.grad_scale * (p.scale[0] / p.sigma[0]) * p.dot[0]; }
     double ss = 0.0;
-    for (long i = (long)b * 256 + threadIdx.x; i < p.n; i += (long)nb * 256) {
-        float g = c0 * p.grad[i];
-        if (p.dsigma) g -= c1 * p.dsigma[i];
-        float u = g;
-        if (p.mom) {
-            const float m = __builtin_fmaf(t.momentum, p.mom[i], g);
-            p.mom_out[i] = m;
-            u = t.nesterov ? __builtin_fmaf(t.momentum, m, g) : m;
-            if (p.u) p.u[i] = u;
+    if (p.vec) {                                             // every pointer 16-byte aligned: four float4 per tensor in flight
+        const long n4 = p.n >> 2;
+        constexpr int U = 4;
+        for (long i0 = (long)b * 256 + threadIdx.x; i0 < n4; i0 += (long)nb * 256 * U) {
+            float4 g[U], d[U], m[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long i = i0 + (long)u * nb * 256;
+                if (i < n4) {
+                    g[u] = reinterpret_cast<const float4 *>(p.grad)[i];
+                    if (p.dsigma) d[u] = reinterpret_cast<const float4 *>(p.dsigma)[i];
+                    if (p.mom) m[u] = reinterpret_cast<const float4 *>(p.mom)[i];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long i = i0 + (long)u * nb * 256;
+                if (i >= n4) break;
+                float gv[4] = {g[u].x, g[u].y, g[u].z, g[u].w}, mv[4] = {m[u].x, m[u].y, m[u].z, m[u].w};
+                const float dv[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    gv[j] *= c0;
+                    if (p.dsigma) gv[j] -= c1 * dv[j];
+                    if (p.mom) {
+                        mv[j] = __builtin_fmaf(t.momentum, mv[j], gv[j]);
+                        gv[j] = t.nesterov ? __builtin_fmaf(t.momentum, mv[j], gv[j]) : mv[j];
+                    }
+                    ss += (double)gv[j] * (double)gv[j];
+                }
+                if (p.mom) {
+                    reinterpret_cast<float4 *>(p.mom_out)[i] = make_float4(mv[0], mv[1], mv[2], mv[3]);
+                    if (p.u) reinterpret_cast<float4 *>(p.u)[i] = make_float4(gv[0], gv[1], gv[2], gv[3]);
+                }
+            }
         }
-        ss += (double)u * (double)u;
     }
+    for (long i = (p.vec ? p.n & ~3L : 0) + (long)b * 256 + threadIdx.x; i < p.n; i += (long)nb * 256)
+        ss += mu_prep_one(p, t, i, p.grad[i], c0, c1, p.dsigma ? p.dsigma[i] : 0.f, p.mom ? p.mom[i] : 0.f);
     ss = wave_sum(ss);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
     __syncthreads();
@@ -179,49 +253,54 @@ struct MuSplit {
     int nparts;
     f16 *x, *xt;                     // [mp, np] and [np, mp]
     int rows, cols, mp, np, tall;    // tall: rows = n
-    unsigned first_block;
 };
-struct MuSplitTable { MuSplit j[kMuGroup]; int n; };
+struct MuSplitTable { MuFirst<kMuGroup> f; MuSplit j[kMuGroup]; };
 
 // one 64 x 64 tile of the padded matrix; "natural" = the operand whose rows are U's rows
 __global__ __launch_bounds__(256) void mu_split_kernel(MuSplitTable t) {
     __shared__ float tile[64][65];
-    __shared__ double s_inv;
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_block) ++q;
+    __shared__ double s_sum[4];
+    const int q = mu_which(t.f, blockIdx.x);
     const MuSplit &p = t.j[q];
-    const int b = blockIdx.x - p.first_block;
+    const int b = blockIdx.x - t.f.first[q];
     const int prows = p.tall ? p.np : p.mp, pcols = p.tall ? p.mp : p.np;
     const int r0 = b / (pcols / 64) * 64, c0 = b % (pcols / 64) * 64;
-    if (threadIdx.x < 64) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < p.nparts; i += 64) s += p.part[i];
-        s = wave_sum(s);
-        if (threadIdx.x == 0) s_inv = s > 0.0 ? (double)kScaleX / sqrt(s) : s == 0.0 ? 0.0 : s;       // NaN stays NaN
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < kMuPrepMax / 256; ++i) {
+        const int at = threadIdx.x + 256 * i;
+        ss += at < p.nparts ? p.part[at] : 0.0;
     }
-    __syncthreads();
-    const double inv = s_inv;
-    const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6;
+    ss = wave_sum(ss);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = ss;
     f16 *nat = p.tall ? p.xt : p.x, *tra = p.tall ? p.x : p.xt;
-    const int ldn = 2 * pcols, ldt = 2 * prows;
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int r = r0 + tr + 4 * i, c = c0 + tc;
-        const float v = r < p.rows && c < p.cols ? (float)((double)p.u[(size_t)r * p.cols + c] * inv) : 0.f;
-        tile[tr + 4 * i][tc] = v;
-        f16 hi, lo;
-        mu_split(v, hi, lo);
-        const size_t o = mu_off(r, c, ldn);
-        nat[o] = hi; nat[o + 32] = lo;
+    {
+        const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6;
+        float u[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = r0 + tr + 4 * i, c = c0 + tc;
+            u[i] = r < p.rows && c < p.cols ? p.u[(size_t)r * p.cols + c] : 0.f;
+        }
+        __syncthreads();
+        const double s = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        const double inv = s > 0.0 ? (double)kScaleX / sqrt(s) : s == 0.0 ? 0.0 : s;                 // (NaN stays NaN)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) tile[tr + 4 * i][tc] = (float)((double)u[i] * inv);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int c = tr + 4 * i;
-        f16 hi, lo;
-        mu_split(tile[tc][c], hi, lo);
-        const size_t o = mu_off(c0 + c, r0 + tc, ldt);
-        tra[o] = hi; tra[o + 32] = lo;
+    // a lane writes 8 values along the operand's own k: lane = row % 32 + 32 * (k / 8 % 2), as the blocks are laid out
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int blk = w * 2 + i, r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[r][k + e];
+        mu_put8(nat, mu_off(r0 + r, c0 + k, pcols / 16), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[k + e][r];
+        mu_put8(tra, mu_off(c0 + r, r0 + k, prows / 16), v);
     }
 }
 
@@ -231,65 +310,69 @@ struct MuGram {
     float *slab;                     // [splits][tiles][128][128]
     f16 *a;                          // [mp, mp]
     int mp, np, tiles, splits, steps_per;
-    unsigned first_block, first_reduce;
 };
-struct MuGramTable { MuGram j[kMuGroup]; int n; };
+struct MuGramTable { MuFirst<kMuGroup> f, r; MuGram j[kMuGroup]; };
 
 __global__ __launch_bounds__(256, 2) void mu_gram_kernel(MuGramTable t) {
-    __shared__ __attribute__((aligned(16))) char lds[MuTile<2>::kLds];
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_block) ++q;
+    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage];
+    const int q = mu_which(t.f, blockIdx.x);
     const MuGram &p = t.j[q];
-    const int b = blockIdx.x - p.first_block, split = b / p.tiles, tile = b % p.tiles;
+    const int b = mu_item(blockIdx.x - t.f.first[q], p.tiles * p.splits);
+    if (b < 0) return;
+    const int split = b / p.tiles, tile = b % p.tiles;
     int ti, tj;
     mu_tri(tile, ti, tj);
     const int s0 = split * p.steps_per, all = p.np / 32;
     const int steps = s0 + p.steps_per < all ? p.steps_per : all - s0;
     f32x16 acc[2][2];
-    mu_tile<2>(p.x + (size_t)ti * 128 * 2 * p.np + (size_t)s0 * 64, 2 * p.np, p.x + (size_t)tj * 128 * 2 * p.np + (size_t)s0 * 64, 2 * p.np,
-               steps, lds, acc);
+    const size_t sx = mu_strip(p.np / 16);
+    mu_tile(p.x + (size_t)ti * 4 * sx + (size_t)s0 * 2048, sx, p.x + (size_t)tj * 4 * sx + (size_t)s0 * 2048, sx, steps, lds, acc);
     float *o = p.slab + ((size_t)split * p.tiles + tile) * 128 * 128;
+    const int w = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[mu_row<2>(i, e) * 128 + mu_col<2>(j)] = acc[i][j][e];
+            for (int e = 0; e < 16; ++e)
+                o[((w >> 1) * 64 + i * 32 + mu_row(e)) * 128 + (w & 1) * 64 + j * 32 + mu_col()] = acc[i][j][e];
 }
 
 // sums the splits of a 32 x 32 block in order, writes A packed, and its mirror image
 __global__ __launch_bounds__(256) void mu_gram_reduce_kernel(MuGramTable t) {
     __shared__ float blk[32][33];
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_reduce) ++q;
+    const int q = mu_which(t.r, blockIdx.x);
     const MuGram &p = t.j[q];
-    const int b = blockIdx.x - p.first_reduce, tile = b >> 4, sub = b & 15;
+    const int b = blockIdx.x - t.r.first[q], tile = b >> 4, sub = b & 15;
     int ti, tj;
     mu_tri(tile, ti, tj);
-    const int r0 = (sub >> 2) * 32, c0 = (sub & 3) * 32, tc = threadIdx.x & 31, tr = threadIdx.x >> 5;
-    const float k = kScaleA / (kScaleX * kScaleX);
+    const int r0 = (sub >> 2) * 32, c0 = (sub & 3) * 32, tc = (threadIdx.x & 7) * 4, tr = threadIdx.x >> 3;
+    const double k = (double)kScaleA / ((double)kScaleX * kScaleX);
+    const float *s = p.slab + (size_t)tile * 128 * 128 + (r0 + tr) * 128 + c0 + tc;
+    const size_t next = (size_t)p.tiles * 128 * 128;
+    double v[4] = {0.0, 0.0, 0.0, 0.0};                      // (the splits' own sums are short: the long one is formed here)
+    for (int z0 = 0; z0 < p.splits; z0 += 8) {
+        float4 f[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = tr + 8 * i;
-        const float *s = p.slab + (size_t)tile * 128 * 128 + (r0 + r) * 128 + c0 + tc;
-        double sum = 0.0;                                    // (the splits' own sums are short: this is where the long one is formed)
-        for (int z = 0; z < p.splits; ++z) sum += (double)s[(size_t)z * p.tiles * 128 * 128];
-        const float v = (float)(sum * k);
-        blk[r][tc] = v;
-        f16 hi, lo;
-        mu_split(v, hi, lo);
-        const size_t o = mu_off(ti * 128 + r0 + r, tj * 128 + c0 + tc, 2 * p.mp);
-        p.a[o] = hi; p.a[o + 32] = lo;
+        for (int z = 0; z < 8; ++z) f[z] = *reinterpret_cast<const float4 *>(s + (size_t)(z0 + z < p.splits ? z0 + z : z0) * next);
+#pragma unroll
+        for (int z = 0; z < 8; ++z)
+            if (z0 + z < p.splits) { v[0] += f[z].x; v[1] += f[z].y; v[2] += f[z].z; v[3] += f[z].w; }
     }
-    if (ti == tj) return;
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = tr + 8 * i;
-        f16 hi, lo;
-        mu_split(blk[tc][c], hi, lo);
-        const size_t o = mu_off(tj * 128 + c0 + c, ti * 128 + r0 + tc, 2 * p.mp);
-        p.a[o] = hi; p.a[o + 32] = lo;
+    for (int e = 0; e < 4; ++e) blk[tr][tc + e] = (float)(v[e] * k);
+    __syncthreads();
+    // waves 0, 1: the block's two 16-column halves; waves 2, 3: its mirror image (a tile on the diagonal holds both halves)
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 31, kk = (w & 1) * 16 + (lane >> 5) * 8, R = ti * 128 + r0, K = tj * 128 + c0;
+    float o[8];
+    if (w < 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = blk[r][kk + e];
+        mu_put8(p.a, mu_off(R + r, K + kk, p.mp / 16), o);
+    } else if (ti != tj) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = blk[kk + e][r];
+        mu_put8(p.a, mu_off(K + r, R + kk, p.mp / 16), o);
     }
 }
 
@@ -300,43 +383,113 @@ struct MuSquare {
     const f16 *z;                    // polynomial form: o += zscale * z + diag on the diagonal; null: the plain product
     float alpha, zscale, diag;
     int mp, tiles;
-    unsigned first_block;
 };
-struct MuSquareTable { MuSquare j[2 * kMuGroup]; int n; };
+struct MuSquareTable { MuFirst<2 * kMuGroup> f; MuSquare j[2 * kMuGroup]; };
 
-__global__ __launch_bounds__(256) void mu_square_kernel(MuSquareTable t) {
-    __shared__ __attribute__((aligned(16))) char lds[MuTile<1>::kLds];
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_block) ++q;
+// Latency-bound (one matrix has 36 tiles at m = 512): no staging, the four waves of a tile take the 32-wide reduction steps in turn,
+// each straight from L2 into MFMA operands with the next step's loads in flight, and their sums meet in LDS.
+__global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
+    __shared__ __attribute__((aligned(16))) float part[4][64 * 64];
+    const int q = mu_which(t.f, blockIdx.x);
     const MuSquare &p = t.j[q];
     int ti, tj;
-    mu_tri(blockIdx.x - p.first_block, ti, tj);
-    const int ld = 2 * p.mp;
-    f32x16 acc[1][1];
-    mu_tile<1>(p.a + (size_t)ti * 64 * ld, ld, p.b + (size_t)tj * 64 * ld, ld, p.mp / 32, lds, acc);
-    const int c = tj * 64 + mu_col<1>(0);
+    const int item = mu_item(blockIdx.x - t.f.first[q], p.tiles);
+    if (item < 0) return;
+    mu_tri(item, ti, tj);
+    const int kb = p.mp / 16, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const size_t sr = mu_strip(kb);
+    const f16 *a = p.a + (size_t)ti * 2 * sr + lane * 8, *b = p.b + (size_t)tj * 2 * sr + lane * 8;
+    f32x16 acc[2][2];
 #pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-        f16x4 hi, lo;
-        const int r = ti * 64 + mu_row<1>(0, e4 * 4);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float v = p.alpha * acc[0][0][e4 * 4 + e];
-            const size_t o = mu_off(r + e, c, ld);
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+    f16x8 fa[2][2][2], fb[2][2][2];                          // [ks][block][hi, lo]
+    auto fetch = [&](int s, f16x8 (&xa)[2][2][2], f16x8 (&xb)[2][2][2]) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    xa[ks][i][h] = *reinterpret_cast<const f16x8 *>(a + i * sr + (size_t)s * 2048 + ks * 1024 + h * 512);
+                    xb[ks][i][h] = *reinterpret_cast<const f16x8 *>(b + i * sr + (size_t)s * 2048 + ks * 1024 + h * 512);
+                }
+    };
+    auto multiply = [&](const f16x8 (&xa)[2][2][2], const f16x8 (&xb)[2][2][2]) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][0], xb[ks][j][1], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][1], xb[ks][j][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][0], xb[ks][j][0], acc[i][j], 0, 0, 0);
+                }
+    };
+    const int steps = p.mp / 32;                             // a multiple of 4: every wave has the same number
+    fetch(w, fa, fb);
+    // 512 pieces of 8 values of a row: block (row block, 16 columns) = w * 2 + i
+    f16x8 zh[2], zl[2];
+    if (p.z) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int blk = w * 2 + i;
+            const size_t o = mu_off(ti * 64 + (blk >> 2) * 32 + (lane & 31), tj * 64 + (blk & 3) * 16 + (lane >> 5) * 8, kb);
+            zh[i] = *reinterpret_cast<const f16x8 *>(p.z + o); zl[i] = *reinterpret_cast<const f16x8 *>(p.z + o + 512);
+        }
+    }
+    for (int s = w; s < steps; s += 4) {
+        f16x8 na[2][2][2], nb[2][2][2];
+        const bool more = s + 4 < steps;
+        if (more) fetch(s + 4, na, nb);
+        multiply(fa, fb);
+        if (more) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) { fa[ks][i][h] = na[ks][i][h]; fb[ks][i][h] = nb[ks][i][h]; }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[w][mu_lds(i * 32 + mu_row(e), j * 32 + mu_col())] = acc[i][j][e];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int blk = w * 2 + i, r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
+        const int at = mu_lds(r, k);
+        const size_t o = mu_off(ti * 64 + r, tj * 64 + k, kb);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = p.alpha * ((part[0][at + e] + part[1][at + e]) + (part[2][at + e] + part[3][at + e]));
             if (p.z) {
-                v += p.zscale * ((float)p.z[o] + (float)p.z[o + 32]);
-                if (r + e == c) v += p.diag;
+                v[e] += p.zscale * ((float)zh[i][e] + (float)zl[i][e]);
+                if (ti * 64 + r == tj * 64 + k + e) v[e] += p.diag;
             }
-            f16 h, l;
-            mu_split(v, h, l);
-            p.o[o] = h; p.o[o + 32] = l;
-            hi[e] = h; lo[e] = l;
         }
+        mu_put8(p.o, o, v);
         if (ti != tj) {
-            const size_t o = mu_off(c, r, ld);
-            *reinterpret_cast<f16x4 *>(p.o + o) = hi;
-            *reinterpret_cast<f16x4 *>(p.o + o + 32) = lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[0][at + e] = v[e];          // (this thread's own piece: nobody else reads it before the barrier)
         }
+    }
+    if (ti == tj) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int blk = w * 2 + i, c = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = part[0][mu_lds(k + e, c)];
+        mu_put8(p.o, mu_off(tj * 64 + c, ti * 64 + k, kb), v);
     }
 }
 
@@ -347,55 +500,73 @@ struct MuApply {
     const float *param;              // last, update form: out = keep * param - step * O; null: out = O
     float *out;                      // last: [rows, cols]
     float alpha, keep, step;
-    int mp, np, rows, cols, tiles_c;
-    unsigned first_block;
+    int mp, np, rows, cols, tiles_m, items, flip;
 };
-struct MuApplyTable { MuApply j[kMuGroup]; int n; };
+struct MuApplyTable { MuFirst<kMuGroup> f; MuApply j[kMuGroup]; };
 
 template <bool LAST>
 __global__ __launch_bounds__(256, 2) void mu_apply_kernel(MuApplyTable t) {
-    __shared__ __attribute__((aligned(16))) char lds[MuTile<2>::kLds];
-    int q = 0;
-    while (q + 1 < t.n && blockIdx.x >= t.j[q + 1].first_block) ++q;
+    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage];
+    const int q = mu_which(t.f, blockIdx.x);
     const MuApply &p = t.j[q];
-    const int b = blockIdx.x - p.first_block, r0 = b / p.tiles_c * 128, c0 = b % p.tiles_c * 128;
+    const int b = mu_item(blockIdx.x - t.f.first[q], p.items), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    if (b < 0) return;
+    // the m side of the tile runs fastest: its operand (P, at most a few MB) stays in L2 while X streams through once
+    const int tr = (LAST && p.flip ? b / p.tiles_m : b % p.tiles_m) * 128, tc = (LAST && p.flip ? b % p.tiles_m : b / p.tiles_m) * 128;
+    const size_t sr = mu_strip(p.mp / 16);
     f32x16 acc[2][2];
-    mu_tile<2>(p.a + (size_t)r0 * 2 * p.mp, 2 * p.mp, p.b + (size_t)c0 * 2 * p.mp, 2 * p.mp, p.mp / 32, lds, acc);
+    mu_tile(p.a + (size_t)(tr / 32) * sr, sr, p.b + (size_t)(tc / 32) * sr, sr, p.mp / 32, lds, acc);
+    const int r0 = tr + (w >> 1) * 64, c0 = tc + (w & 1) * 64;           // this wave's 64 x 64
+    if (LAST) {
+        // (every parameter is read before the first result is written: out may be param)
+        float old[2][2][16];
+        if (p.param) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int r = r0 + i * 32 + mu_row(e), c = c0 + j * 32 + mu_col();
+                        old[i][j][e] = r < p.rows && c < p.cols ? p.param[(size_t)r * p.cols + c] : 0.f;
+                    }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = r0 + i * 32 + mu_row(e), c = c0 + j * 32 + mu_col();
+                    const float v = p.alpha * acc[i][j][e];
+                    if (r < p.rows && c < p.cols) p.out[(size_t)r * p.cols + c] = p.param ? p.keep * old[i][j][e] - p.step * v : v;
+                }
+        return;
+    }
+    // both layouts of the next X from the wave's own quarter of the staging buffers (mu_tile ends with a barrier)
+    float *mine = reinterpret_cast<float *>(lds) + w * 4096;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int c = c0 + mu_col<2>(j);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                f16x4 hi, lo;
-                const int r = r0 + mu_row<2>(i, e4 * 4);
+            for (int e = 0; e < 16; ++e) mine[mu_lds(i * 32 + mu_row(e), j * 32 + mu_col())] = p.alpha * acc[i][j][e];
+    __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = p.alpha * acc[i][j][e4 * 4 + e];
-                    if (LAST) {
-                        if (r + e < p.rows && c < p.cols) {
-                            const size_t o = (size_t)(r + e) * p.cols + c;
-                            p.out[o] = p.param ? p.keep * p.param[o] - p.step * v : v;
-                        }
-                    } else {
-                        f16 h, l;
-                        mu_split(v, h, l);
-                        const size_t o = mu_off(r + e, c, 2 * p.np);
-                        p.x[o] = h; p.x[o + 32] = l;
-                        hi[e] = h; lo[e] = l;
-                    }
-                }
-                if (!LAST) {
-                    const size_t o = mu_off(c, r, 2 * p.mp);
-                    *reinterpret_cast<f16x4 *>(p.xt + o) = hi;
-                    *reinterpret_cast<f16x4 *>(p.xt + o + 32) = lo;
-                }
-            }
-        }
+    for (int blk = 0; blk < 8; ++blk) {
+        const int r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mine[mu_lds(r, k) + e];
+        mu_put8(p.x, mu_off(r0 + r, c0 + k, p.np / 16), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mine[mu_lds(k + e, r)];
+        mu_put8(p.xt, mu_off(c0 + r, r0 + k, p.mp / 16), v);
+    }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
+static bool mu_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 struct MuMat {                       // a matrix's place in the workspace
     int rows, cols, mp, np, tall, nparts, tiles, splits, steps_per;
     size_t part, u, x, xt, xt2, a, qq, w, p0, p1, slab;      // byte offsets
@@ -410,22 +581,22 @@ static MuMat mu_place(int rows, int cols, bool keep_u, int steps, size_t base) {
     m.np = (int)(((long)l + kMuPad - 1) / kMuPad * kMuPad);
     const long n = (long)rows * cols, want = (n + kMuPrepPer - 1) / kMuPrepPer;
     m.nparts = (int)(want < kMuPrepMax ? want : kMuPrepMax);
-    // one triangle of 128 x 128 tiles; the reduction split so that a matrix alone gives about 512 workgroups, at least four
-    // 32-wide steps each
+    // one triangle of 128 x 128 tiles, the reduction in runs of 8 to 16 32-wide steps: 512 workgroups from one matrix where it has
+    // them, and no run so short that its 64 KB of sums cost more than its 32 KB stages.  (A rule on the matrix alone: what it
+    // gives does not depend on the others of a call.)
     const int tb = m.mp / 128, all = m.np / 32;
     m.tiles = tb * (tb + 1) / 2;
-    int splits = (512 + m.tiles - 1) / m.tiles;
-    if (splits > all / 4) splits = all / 4;
-    if (splits < 1) splits = 1;
-    m.steps_per = (all + splits - 1) / splits;
+    long run = ((long)m.tiles * all + 511) / 512;
+    run = run < 8 ? 8 : run > 16 ? 16 : (run + 1) & ~1L;     // (even: mu_tile)
+    m.steps_per = all < run ? all : (int)run;
     m.splits = (all + m.steps_per - 1) / m.steps_per;
-    const size_t big = mu_round((size_t)m.mp * m.np * 4), sq = mu_round((size_t)m.mp * m.mp * 4);
+    const size_t bx = m.mp / 32 * mu_strip(m.np / 16) * 2, bt = m.np / 32 * mu_strip(m.mp / 16) * 2, sq = m.mp / 32 * mu_strip(m.mp / 16) * 2;
     size_t o = mu_round(base);
     auto take = [&](size_t bytes) { const size_t at = o; o += mu_round(bytes); return at; };
     m.part = take((size_t)m.nparts * sizeof(double));
     m.u = keep_u ? take((size_t)n * 4) : 0;
-    m.x = take(big); m.xt = take(big);
-    m.xt2 = steps > kMuChain ? take(big) : 0;
+    m.x = take(bx); m.xt = take(bt);
+    m.xt2 = steps > kMuChain ? take(bt) : 0;
     m.a = take(sq); m.qq = take(sq); m.w = take(sq); m.p0 = take(sq); m.p1 = take(sq);
     m.slab = take((size_t)m.splits * m.tiles * 128 * 128 * 4);
     m.end = o;
@@ -440,6 +611,17 @@ struct MuJob {
     float keep, step;
 };
 
+// the matrices with the longest products first: a launch ends with its short workgroups
+static void mu_order(MuJob *j, int n) {
+    std::stable_sort(j, j + n, [](const MuJob &a, const MuJob &b) {
+        const int sa = a.rows < a.cols ? a.rows : a.cols, sb = b.rows < b.cols ? b.rows : b.cols;
+        return sa != sb ? sa > sb : (long)a.rows * a.cols > (long)b.rows * b.cols;
+    });
+}
+template <int N> static void mu_close(MuFirst<N> &f, int n) {
+    for (int i = n; i < N; ++i) f.first[i] = 0xffffffffu;
+}
+
 // all matrices of one group, phase by phase
 static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, int nesterov, float grad_scale, int steps, char *ws,
                         hipStream_t st) {
@@ -449,7 +631,7 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
     for (int i = 0; i < n; ++i) { m[i] = mu_place(jobs[i].rows, jobs[i].cols, keep_u, steps, at); at = m[i].end; }
     {
         MuPrepTable t{};
-        t.n = n; t.momentum = momentum; t.grad_scale = grad_scale; t.nesterov = nesterov;
+        t.momentum = momentum; t.grad_scale = grad_scale; t.nesterov = nesterov;
         unsigned blocks = 0;
         for (int i = 0; i < n; ++i) {
             MuPrep &p = t.j[i];
@@ -458,15 +640,17 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             p.dsigma = jobs[i].dsigma; p.dot = jobs[i].dot; p.sigma = jobs[i].sigma; p.scale = jobs[i].scale;
             p.part = (double *)(ws + m[i].part);
             p.n = (long)jobs[i].rows * jobs[i].cols;
-            p.first_block = blocks;
+            p.vec = mu_aligned(p.grad) && mu_aligned(p.mom) && mu_aligned(p.mom_out) && mu_aligned(p.dsigma);
+            p.blocks = m[i].nparts;
+            t.f.first[i] = blocks;
             blocks += m[i].nparts;
         }
+        mu_close(t.f, n);
         hipLaunchKernelGGL(mu_prep_kernel, dim3(blocks), dim3(256), 0, st, t);
     }
     f16 *x[kMuGroup], *xt[kMuGroup], *xt_next[kMuGroup];
     {
         MuSplitTable t{};
-        t.n = n;
         unsigned blocks = 0;
         for (int i = 0; i < n; ++i) {
             MuSplit &p = t.j[i];
@@ -475,24 +659,26 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             x[i] = (f16 *)(ws + m[i].x); xt[i] = (f16 *)(ws + m[i].xt); xt_next[i] = (f16 *)(ws + m[i].xt2);
             p.x = x[i]; p.xt = xt[i];
             p.rows = jobs[i].rows; p.cols = jobs[i].cols; p.mp = m[i].mp; p.np = m[i].np; p.tall = m[i].tall;
-            p.first_block = blocks;
+            t.f.first[i] = blocks;
             blocks += (unsigned)((long)m[i].mp / 64 * (m[i].np / 64));
         }
+        mu_close(t.f, n);
         hipLaunchKernelGGL(mu_split_kernel, dim3(blocks), dim3(256), 0, st, t);
     }
     for (int done = 0; done < steps;) {
         const int chain = steps - done < kMuChain ? steps - done : kMuChain;
         {
             MuGramTable t{};
-            t.n = n;
-            unsigned blocks = 0, red = 0;
+                unsigned blocks = 0, red = 0;
             for (int i = 0; i < n; ++i) {
                 MuGram &p = t.j[i];
                 p.x = x[i]; p.slab = (float *)(ws + m[i].slab); p.a = (f16 *)(ws + m[i].a);
                 p.mp = m[i].mp; p.np = m[i].np; p.tiles = m[i].tiles; p.splits = m[i].splits; p.steps_per = m[i].steps_per;
-                p.first_block = blocks; p.first_reduce = red;
-                blocks += p.tiles * p.splits; red += p.tiles * 16;
+                t.f.first[i] = blocks; t.r.first[i] = red;
+                blocks += (p.tiles * p.splits + 7) & ~7; red += p.tiles * 16;
             }
+            mu_close(t.f, n);
+            mu_close(t.r, n);
             hipLaunchKernelGGL(mu_gram_kernel, dim3(blocks), dim3(256), 0, st, t);
             hipLaunchKernelGGL(mu_gram_reduce_kernel, dim3(red), dim3(256), 0, st, t);
         }
@@ -503,20 +689,23 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             const float sp = k == 1 ? kScaleQ : kScaleP;     // scale of the P that this step's Q multiplies
             MuSquareTable t{};
             unsigned blocks = 0;
+            int nt = 0;
             auto add = [&](int i, size_t a, size_t b, size_t o, float alpha) -> MuSquare & {
-                MuSquare &p = t.j[t.n++];
+                MuSquare &p = t.j[nt];
+                p = MuSquare{};
                 p.a = (const f16 *)(ws + a); p.b = (const f16 *)(ws + b); p.o = (f16 *)(ws + o); p.alpha = alpha;
                 p.mp = m[i].mp;
                 const int tb = p.mp / 64;
                 p.tiles = tb * (tb + 1) / 2;
-                p.first_block = blocks;
-                blocks += p.tiles;
+                t.f.first[nt++] = blocks;
+                blocks += (p.tiles + 7) & ~7;
                 return p;
             };
             auto go = [&]() {
-                if (t.n) hipLaunchKernelGGL(mu_square_kernel, dim3(blocks), dim3(256), 0, st, t);
-                t = MuSquareTable{};
+                mu_close(t.f, nt);
+                if (nt) hipLaunchKernelGGL(mu_square_kernel, dim3(blocks), dim3(256), 0, st, t);
                 blocks = 0;
+                nt = 0;
             };
             auto q_of = [&](int i) { return k == 0 ? m[i].p0 : m[i].qq; };
             for (int i = 0; i < n; ++i) {                    // Q = a I + b A + c A^2
@@ -537,7 +726,6 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
         }
         done += chain;
         MuApplyTable t{};
-        t.n = n;
         unsigned blocks = 0;
         const float sp = chain == 1 ? kScaleQ : kScaleP;
         for (int i = 0; i < n; ++i) {
@@ -546,13 +734,15 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             const bool flip = done == steps && m[i].tall;    // the result in U's own layout: tile rows along its rows
             p.a = flip ? xt[i] : pp; p.b = flip ? pp : xt[i];
             p.mp = m[i].mp; p.np = m[i].np; p.rows = jobs[i].rows; p.cols = jobs[i].cols;
-            p.tiles_c = (flip ? m[i].mp : m[i].np) / 128;
+            p.tiles_m = m[i].mp / 128; p.flip = flip;
             p.alpha = done == steps ? 1.f / (sp * kScaleX) : 1.f / sp;
             p.x = x[i]; p.xt = xt_next[i];
             p.param = update ? jobs[i].param : nullptr; p.out = jobs[i].out; p.keep = jobs[i].keep; p.step = jobs[i].step;
-            p.first_block = blocks;
-            blocks += (unsigned)((long)m[i].mp / 128 * (m[i].np / 128));
+            t.f.first[i] = blocks;
+            p.items = m[i].mp / 128 * (m[i].np / 128);
+            blocks += (unsigned)(p.items + 7) & ~7u;
         }
+        mu_close(t.f, n);
         if (done == steps) hipLaunchKernelGGL((mu_apply_kernel<true>), dim3(blocks), dim3(256), 0, st, t);
         else hipLaunchKernelGGL((mu_apply_kernel<false>), dim3(blocks), dim3(256), 0, st, t);
         for (int i = 0; i < n; ++i) { f16 *s = xt[i]; xt[i] = xt_next[i]; xt_next[i] = s; }
@@ -607,6 +797,7 @@ extern "C" int mmdgan_orthogonalize(const mmdgan_muon_job *jobs, int n_jobs, int
         for (int i = g; i < n_jobs && n < kMuGroup; ++i, ++n) {
             j[n].rows = jobs[i].rows; j[n].cols = jobs[i].cols; j[n].grad = jobs[i].grad; j[n].out = jobs[i].out;
         }
+        mu_order(j, n);
         if (int rc = mu_run_group(j, n, false, 0.f, 0, 1.f, steps, (char *)workspace, (hipStream_t)stream)) return rc;
     }
     return MMDGAN_OK;
@@ -627,6 +818,7 @@ extern "C" int mmdgan_muon_update(const mmdgan_muon_job *jobs, int n_jobs, float
             d.keep = (float)(1.0 - (double)lr * weight_decay);
             d.step = (float)((double)lr * 0.2 * sqrt((double)big));
         }
+        mu_order(j, n);
         if (int rc = mu_run_group(j, n, true, momentum, nesterov != 0, grad_scale, steps, (char *)workspace, (hipStream_t)stream)) return rc;
     }
     return MMDGAN_OK;
