@@ -17,12 +17,10 @@
 // Layout ("packed"): an [R, K] operand is cut into 32 x 16 blocks, row blocks outermost; a block is 2 KB: the 64 lanes' 16-byte
 // MFMA operands of the hi parts in lane order (lane = row % 32 + 32 * (k / 8 % 2), 8 halves along k), then those of the lo parts.
 // Every operand load of a wave is one contiguous kilobyte, from L2 or from LDS, without bank conflicts or swizzles.  All sides are
-// padded to 128 with zeros, so the products have no edges.  Row blocks lie 4 KB further apart than their blocks fill: with m a
+// padded to 128 with zeros, so the products have no edges.  (Matrices with a side of 64 or less: muon_small.hip.)  Row blocks lie 4 KB further apart than their blocks fill: with m a
 // power of two all workgroups of a product, at the same reduction step, would otherwise read addresses that are equal modulo
 // 128 KB, from the same few memory channels.
-#include "common.h"
-
-#include <algorithm>
+#include "muon_internal.h"
 
 namespace mmdgan {
 
@@ -32,10 +30,8 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int mu_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMuGroup = 16;                 // matrices per launch (the task tables travel by value)
 constexpr int kMuPad = 128;
 constexpr int kMuChain = 3;                  // steps between two true Gram matrices
-constexpr float kMuA = 3.4445f, kMuB = -4.7750f, kMuC = 2.0315f;
 constexpr float kScaleX = 4096.f, kScaleA = 4096.f, kScaleQ = 8192.f, kScaleP = 1024.f;
 
 // halves from one row block to the next, of `kb` = K / 16 blocks
@@ -152,17 +148,6 @@ __device__ __forceinline__ void mu_tri(int t, int &ti, int &tj) {
 __device__ __forceinline__ int mu_item(unsigned b, unsigned n) {
     const unsigned x = b & 7, per = n >> 3, rest = n & 7, i = b >> 3;
     return i < per + (x < rest ? 1u : 0u) ? (int)(x * per + (x < rest ? x : rest) + i) : -1;
-}
-
-// Which matrix of a launch a workgroup belongs to: `first` holds the matrices' first workgroups (entries beyond the last: none
-// reaches them).  Kept apart from the jobs, in two cache lines at most: a search through the jobs themselves waited for one
-// kernel-argument line after the other.
-template <int N> struct MuFirst { unsigned first[N]; };
-template <int N> __device__ __forceinline__ int mu_which(const MuFirst<N> &f, unsigned b) {
-    int q = 0;
-#pragma unroll
-    for (int i = 1; i < N; ++i) q += b >= f.first[i] ? 1 : 0;
-    return q;
 }
 
 // ---- momentum and norm -------------------------------------------------------------------------------------------
@@ -572,7 +557,6 @@ struct MuMat {                       // a matrix's place in the workspace
     size_t part, u, x, xt, xt2, a, qq, w, p0, p1, slab;      // byte offsets
     size_t end;
 };
-static size_t mu_round(size_t v) { return (v + 255) & ~(size_t)255; }
 static MuMat mu_place(int rows, int cols, bool keep_u, int steps, size_t base) {
     MuMat m{};
     m.rows = rows; m.cols = cols; m.tall = rows >= cols;
@@ -603,35 +587,30 @@ static MuMat mu_place(int rows, int cols, bool keep_u, int steps, size_t base) {
     return m;
 }
 
-struct MuJob {
-    int rows, cols;
-    const float *grad, *mom, *param;
-    float *mom_out, *out;
-    const float *dsigma, *dot, *sigma, *scale;
-    float keep, step;
-};
-
 // the matrices with the longest products first: a launch ends with its short workgroups
 static void mu_order(MuJob *j, int n) {
-    std::stable_sort(j, j + n, [](const MuJob &a, const MuJob &b) {
+    auto before = [](const MuJob &a, const MuJob &b) {
         const int sa = a.rows < a.cols ? a.rows : a.cols, sb = b.rows < b.cols ? b.rows : b.cols;
         return sa != sb ? sa > sb : (long)a.rows * a.cols > (long)b.rows * b.cols;
-    });
-}
-template <int N> static void mu_close(MuFirst<N> &f, int n) {
-    for (int i = n; i < N; ++i) f.first[i] = 0xffffffffu;
+    };
+    for (int i = 1; i < n; ++i) {
+        const MuJob x = j[i];
+        int k = i;
+        for (; k > 0 && before(x, j[k - 1]); --k) j[k] = j[k - 1];
+        j[k] = x;
+    }
 }
 
 // all matrices of one group, phase by phase
-static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, int nesterov, float grad_scale, int steps, char *ws,
-                        hipStream_t st) {
+static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp, char *ws, hipStream_t st) {
     MuMat m[kMuGroup];
-    const bool keep_u = update && nesterov;
+    const int steps = sp.steps;
+    const bool keep_u = update && sp.nesterov;
     size_t at = 0;
     for (int i = 0; i < n; ++i) { m[i] = mu_place(jobs[i].rows, jobs[i].cols, keep_u, steps, at); at = m[i].end; }
     {
         MuPrepTable t{};
-        t.momentum = momentum; t.grad_scale = grad_scale; t.nesterov = nesterov;
+        t.momentum = sp.momentum; t.grad_scale = sp.grad_scale; t.nesterov = sp.nesterov;
         unsigned blocks = 0;
         for (int i = 0; i < n; ++i) {
             MuPrep &p = t.j[i];
@@ -686,7 +665,7 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
         bool in_p0 = true;
         for (int k = 0; k < chain; ++k) {
             const bool last = k == chain - 1;
-            const float sp = k == 1 ? kScaleQ : kScaleP;     // scale of the P that this step's Q multiplies
+            const float s_p = k == 1 ? kScaleQ : kScaleP;    // scale of the P that this step's Q multiplies
             MuSquareTable t{};
             unsigned blocks = 0;
             int nt = 0;
@@ -715,7 +694,7 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             go();
             for (int i = 0; i < n; ++i) {
                 if (!last) add(i, q_of(i), m[i].a, m[i].w, 1.f / kScaleQ);                                     // W = Q A
-                if (k > 0) add(i, m[i].qq, in_p0 ? m[i].p0 : m[i].p1, in_p0 ? m[i].p1 : m[i].p0, kScaleP / (kScaleQ * sp));   // P = Q P
+                if (k > 0) add(i, m[i].qq, in_p0 ? m[i].p0 : m[i].p1, in_p0 ? m[i].p1 : m[i].p0, kScaleP / (kScaleQ * s_p));   // P = Q P
             }
             go();
             if (k > 0) in_p0 = !in_p0;
@@ -727,7 +706,7 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
         done += chain;
         MuApplyTable t{};
         unsigned blocks = 0;
-        const float sp = chain == 1 ? kScaleQ : kScaleP;
+        const float s_p = chain == 1 ? kScaleQ : kScaleP;
         for (int i = 0; i < n; ++i) {
             MuApply &p = t.j[i];
             const f16 *pp = (const f16 *)(ws + (in_p0 ? m[i].p0 : m[i].p1));
@@ -735,7 +714,7 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
             p.a = flip ? xt[i] : pp; p.b = flip ? pp : xt[i];
             p.mp = m[i].mp; p.np = m[i].np; p.rows = jobs[i].rows; p.cols = jobs[i].cols;
             p.tiles_m = m[i].mp / 128; p.flip = flip;
-            p.alpha = done == steps ? 1.f / (sp * kScaleX) : 1.f / sp;
+            p.alpha = done == steps ? 1.f / (s_p * kScaleX) : 1.f / s_p;
             p.x = x[i]; p.xt = xt_next[i];
             p.param = update ? jobs[i].param : nullptr; p.out = jobs[i].out; p.keep = jobs[i].keep; p.step = jobs[i].step;
             t.f.first[i] = blocks;
@@ -747,17 +726,38 @@ static int mu_run_group(const MuJob *jobs, int n, bool update, float momentum, i
         else hipLaunchKernelGGL((mu_apply_kernel<false>), dim3(blocks), dim3(256), 0, st, t);
         for (int i = 0; i < n; ++i) { f16 *s = xt[i]; xt[i] = xt_next[i]; xt_next[i] = s; }
     }
-    return check_launch(update ? "muon_update" : "orthogonalize");
 }
 
-static size_t mu_bytes(const mmdgan_muon_job *jobs, int n, int steps, bool keep_u) {
-    size_t most = 0;
-    for (int g = 0; g < n; g += kMuGroup) {
-        size_t at = 0;
-        for (int i = g; i < n && i < g + kMuGroup; ++i) at = mu_place(jobs[i].rows, jobs[i].cols, keep_u, steps, at).end;
-        if (at > most) most = at;
+// The matrices of a call in groups of kMuGroup, small ones (muon_small.hip) and others each among themselves: calls
+// f(indices, count, small) per group, in an order that depends on the sizes' kinds alone.
+template <typename F> static void mu_groups(const mmdgan_muon_job *jobs, int n, F &&f) {
+    for (int small = 0; small < 2; ++small) {
+        int idx[kMuGroup], k = 0;
+        for (int i = 0; i < n; ++i) {
+            if (mu_is_small(jobs[i].rows, jobs[i].cols) != (small != 0)) continue;
+            idx[k++] = i;
+            if (k == kMuGroup) { f(idx, k, small != 0); k = 0; }
+        }
+        if (k) f(idx, k, small != 0);
     }
+}
+// groups run one after the other in the same scratch
+static size_t mu_bytes(const mmdgan_muon_job *jobs, int n, int steps, bool keep_u) {
+    size_t most = 256;
+    mu_groups(jobs, n, [&](const int *idx, int k, bool small) {
+        size_t at = 0;
+        for (int i = 0; i < k; ++i) {
+            const mmdgan_muon_job &j = jobs[idx[i]];
+            at = small ? mu_round(at) + mu_small_bytes(j.rows, j.cols, keep_u) : mu_place(j.rows, j.cols, keep_u, steps, at).end;
+        }
+        if (at > most) most = at;
+    });
     return most;
+}
+static void mu_run(MuJob *j, int n, bool update, const MuStep &s, bool small, char *ws, hipStream_t st) {
+    mu_order(j, n);
+    if (small) mu_small_run(j, n, s, ws, st);
+    else mu_run_group(j, n, update, s, ws, st);
 }
 static bool mu_sizes_ok(const mmdgan_muon_job *jobs, int n, int steps) {
     if (!jobs || n < 1 || steps < 1 || steps > 16) return false;
@@ -791,35 +791,34 @@ static int mu_check(const mmdgan_muon_job *jobs, int n_jobs, int steps, bool upd
 
 extern "C" int mmdgan_orthogonalize(const mmdgan_muon_job *jobs, int n_jobs, int steps, void *workspace, void *stream) {
     if (int rc = mu_check(jobs, n_jobs, steps, false, workspace, "orthogonalize")) return rc;
-    for (int g = 0; g < n_jobs; g += kMuGroup) {
+    const MuStep s{0.f, 1.f, 0, steps};
+    mu_groups(jobs, n_jobs, [&](const int *idx, int n, bool small) {
         MuJob j[kMuGroup] = {};
-        int n = 0;
-        for (int i = g; i < n_jobs && n < kMuGroup; ++i, ++n) {
-            j[n].rows = jobs[i].rows; j[n].cols = jobs[i].cols; j[n].grad = jobs[i].grad; j[n].out = jobs[i].out;
+        for (int i = 0; i < n; ++i) {
+            const mmdgan_muon_job &q = jobs[idx[i]];
+            j[i].rows = q.rows; j[i].cols = q.cols; j[i].grad = q.grad; j[i].out = q.out;
         }
-        mu_order(j, n);
-        if (int rc = mu_run_group(j, n, false, 0.f, 0, 1.f, steps, (char *)workspace, (hipStream_t)stream)) return rc;
-    }
-    return MMDGAN_OK;
+        mu_run(j, n, false, s, small, (char *)workspace, (hipStream_t)stream);
+    });
+    return check_launch("orthogonalize");
 }
 
 extern "C" int mmdgan_muon_update(const mmdgan_muon_job *jobs, int n_jobs, float lr, float momentum, int nesterov, float weight_decay,
                                   float grad_scale, int apply_fixup, int steps, void *workspace, void *stream) {
     if (int rc = mu_check(jobs, n_jobs, steps, true, workspace, "muon_update")) return rc;
-    for (int g = 0; g < n_jobs; g += kMuGroup) {
+    const MuStep st{momentum, grad_scale, nesterov != 0, steps};
+    mu_groups(jobs, n_jobs, [&](const int *idx, int n, bool small) {
         MuJob j[kMuGroup] = {};
-        int n = 0;
-        for (int i = g; i < n_jobs && n < kMuGroup; ++i, ++n) {
-            const mmdgan_muon_job &s = jobs[i];
-            MuJob &d = j[n];
-            d.rows = s.rows; d.cols = s.cols; d.grad = s.grad; d.mom = s.momentum; d.mom_out = s.momentum_out; d.param = s.param; d.out = s.out;
-            if (apply_fixup && s.dsigma) { d.dsigma = s.dsigma; d.dot = s.dot; d.sigma = s.sigma; d.scale = s.scale; }
-            const int big = s.rows > s.cols ? s.rows : s.cols;
+        for (int i = 0; i < n; ++i) {
+            const mmdgan_muon_job &q = jobs[idx[i]];
+            MuJob &d = j[i];
+            d.rows = q.rows; d.cols = q.cols; d.grad = q.grad; d.mom = q.momentum; d.mom_out = q.momentum_out; d.param = q.param; d.out = q.out;
+            if (apply_fixup && q.dsigma) { d.dsigma = q.dsigma; d.dot = q.dot; d.sigma = q.sigma; d.scale = q.scale; }
+            const int big = q.rows > q.cols ? q.rows : q.cols;
             d.keep = (float)(1.0 - (double)lr * weight_decay);
             d.step = (float)((double)lr * 0.2 * sqrt((double)big));
         }
-        mu_order(j, n);
-        if (int rc = mu_run_group(j, n, true, momentum, nesterov != 0, grad_scale, steps, (char *)workspace, (hipStream_t)stream)) return rc;
-    }
-    return MMDGAN_OK;
+        mu_run(j, n, true, st, small, (char *)workspace, (hipStream_t)stream);
+    });
+    return check_launch("muon_update");
 }
