@@ -22,7 +22,7 @@ from mmdgan_hip.tape import TapeEngine, needs_tape_engine
 class SNGan(object):
     def __init__(self, architecture, num_class=0, loss_type='logistic', optimizer='adam', do_summary=True,
                  do_summary_image=True, num_summary_image=8, image_transpose=False, **kwargs):
-        self.optimizer_type = ['sgd', 'momentum', 'adam', 'rmsprop']
+        self.optimizer_type = ['sgd', 'momentum', 'adam', 'rmsprop', 'muon']
         self.data_format = FLAGS.IMAGE_FORMAT
         self.architecture, self.loss_type, self.optimizer = architecture, loss_type, optimizer
         self.num_class = num_class
@@ -44,7 +44,7 @@ class SNGan(object):
             raise NotImplementedError('conditional models are outside the hot path')
         if loss_type not in ops.LOSS:
             raise NotImplementedError('Not implemented.')                      # math_func.py:2651
-        if optimizer != 'adam':
+        if optimizer not in ('adam', 'muon'):            # 'muon' (orthogonalised updates of the kernels) is not the reference's
             raise NotImplementedError('only the adam branch of opt_config is on the hot path (graph_func.py:518-527)')
         self.engine = None
         self.dist_group = kwargs.get('dist_group')
@@ -53,12 +53,15 @@ class SNGan(object):
     def init_net(self, lr_list, batch_size, seed=0):
         """G and D with their optimisers (my_sngan.py:85-108, 412-415)."""
         if self.engine is None or self.engine.B != batch_size:
-            # residual blocks / scaling ops / identity layers / batch norm in D: the primitive-op engine (mmdgan_hip/tape.py)
-            engine_cls = TapeEngine if needs_tape_engine(self.architecture) else GanEngine
+            # residual blocks / scaling ops / identity layers / batch norm in D / group norm: the primitive-op engine
+            # (mmdgan_hip/tape.py); it has the optimizer 'muon' too
+            tape = self.optimizer == 'muon' or needs_tape_engine(self.architecture)
+            engine_cls = TapeEngine if tape else GanEngine
             self.engine = engine_cls(self.architecture, self.loss_type, lr_list, tuple(self.rep_weights),
                                     batch_size=batch_size, seed=seed, dist_group=self.dist_group,
                                     sn_mode=FLAGS.SPECTRAL_NORM_MODE,                # layer_func.py:802-814
                                     weight_init=FLAGS.WEIGHT_INITIALIZER,           # layer_func.py:27-64
+                                    **({'optimizer': self.optimizer} if tape else {}),
                                     # (how a step reaches the GPU - eager issue, one hipGraph, the library's launch
                                     # plan - is the engine's `launch_mode`; MMDGAN_LAUNCH_MODE, mmdgan_hip/settings.py)
                                     )

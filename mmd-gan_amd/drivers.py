@@ -37,6 +37,8 @@ def run(dataset, argv=None):
     ap.add_argument('--rounds', type=int, default=8)
     ap.add_argument('--loss', default='rep', help="'rep', 'rmb', 'mmd_g', 'mgb', 'hinge', 'logistic'")
     ap.add_argument('--sn-mode', default='default', help="'default' (PICO) or 'sn_paper' (PIM)")
+    ap.add_argument('--optimizer', default='adam', choices=['adam', 'muon'],
+                    help="'muon': the kernels' updates are orthogonalised momentum (the reference has adam)")
     args = ap.parse_args(argv)
     exp = EXPERIMENTS[dataset]
 
@@ -51,14 +53,14 @@ def run(dataset, argv=None):
     architecture, lr_list = configs.CONFIGS[exp.config]()
     rep_weights = [0.0, -1.0]                         # weights of e_kxy and -e_kyy; they must differ by one
     act_k = architecture['discriminator'][0]['act_k']
-    folder = sub_folder_name(args.loss, lr_list, act_k, rep_weights)
+    folder = sub_folder_name(args.loss, lr_list, act_k, rep_weights) + ('' if args.optimizer == 'adam' else '_' + args.optimizer)
     codes = np.random.randn(400, architecture['code'][0][0]).astype(np.float32)      # the same codes every round
 
     # a single record file is named after the dataset, several are <dataset>_000, <dataset>_001, ...
     files = dataset if exp.num_file == 1 else ['{}_{:03d}'.format(dataset, i) for i in range(exp.num_file)]
     num_instance = exp.num_file * exp.per_file
     agent = Agent(files, folder, load_ckpt=True, do_save=True, query_step=1000, print_loss=True)
-    model = SNGan(architecture, num_class=0, loss_type=args.loss, optimizer='adam', rep_weights=rep_weights)
+    model = SNGan(architecture, num_class=0, loss_type=args.loss, optimizer=args.optimizer, rep_weights=rep_weights)
     for _ in range(args.rounds):
         model.training(files, agent, num_instance, lr_list, end_lr=1e-7, max_step=args.steps,
                        batch_size=exp.batch_size, num_threads=7)

@@ -1475,6 +1475,8 @@ class GanEngine:
                 'loss_state': self._loss.state_dict(), 'adam_m': m, 'adam_v': v, 'adam_t': t}
 
     def load_state_dict(self, sd):
+        if sd.get('optimizer', 'adam') != 'adam':                        # (TapeEngine's 'muon': its momentum is no first moment)
+            raise ValueError('the checkpoint is of optimizer {}, this engine runs adam'.format(sd['optimizer']))
         self.set_variables(sd['variables'])
         self.global_step = int(sd['global_step'])
         self._loss.load_state_dict(sd.get('loss_state', {}))

@@ -797,7 +797,7 @@ class AdamArena:
                 segs[i].dsigma, segs[i].dot = sn['dsigma'].data_ptr(), sn['dot'].data_ptr()
                 segs[i].sigma, segs[i].scale = sn['sigma'].data_ptr(), sn['scale'].data_ptr()
             blocks += [(i, b) for b in range((int(n) + 1023) // 1024)]
-        raw = bytes(segs)
+        raw = bytes(segs) or bytes(16)                   # (a net whose every variable is somebody else's: nothing to update)
         self.segs = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(dev)
         self.blocks = torch.tensor(blocks, dtype=torch.int32, device=dev).contiguous()
         self.n_segs, self.n_blocks = len(segments), len(blocks)
@@ -818,6 +818,8 @@ class AdamArena:
     def step(self, lr, step=None, beta1=0.5, beta2=0.999, eps=1e-8, grad_scale=1.0):
         lib = require_device()
         pre, self.prepared = self.prepared, False
+        if self.n_blocks == 0:
+            return
         check(lib.mmdgan_adam_segments(_p(self.params), _p(self.grads), _p(self.m), _p(self.v), self.segs.data_ptr(),
                                        self.n_segs, self.blocks.data_ptr(), self.n_blocks, float(lr), float(beta1),
                                        float(beta2), float(eps), -1 if pre else int(step or 0),

@@ -23,18 +23,19 @@ from .engine import _Arena, _chw_perm, _trunc_normal
 
 _TEMPLATE = {'name': None, 'type': 'default', 'op': 'c', 'out': None, 'bias': 'b', 'act': 'linear', 'act_nm': None,
              'act_k': False, 'w_nm': None, 'w_p': None, 'kernel': 3, 'strides': 1, 'dilation': 1, 'padding': 'SAME',
-             'scale': None, 'in_reshape': None, 'out_reshape': None, 'aux': None}
+             'scale': None, 'in_reshape': None, 'out_reshape': None, 'aux': None, 'groups': None}
 RES_TYPES = ('res', 'res_i', 'res_v1')                                   # layer_func.py:2062
 _PIM = ('sn_paper', 'PIM', 'pim')
+_BN, _GN = ('bn', 'BN'), ('gn', 'GN')        # 'act_nm': the reference's batch norm; group norm (this library's addition)
 
 
 def needs_primitive_ops(designs):
     """a net the hand-scheduled chain does not express: residual blocks, identity layers, scaling ops, an input reshape,
-    'VALID' padding, dilation"""
+    'VALID' padding, dilation, group norm"""
     def plain(v, default):
         return all(x == default for x in v) if isinstance(v, (list, tuple)) else v == default
     return any(d.get('type', 'default') in RES_TYPES or d.get('op') == 'i' or d.get('scale') is not None
-               or d.get('in_reshape') is not None or not plain(d.get('dilation', 1), 1) or not plain(d.get('padding', 'SAME'), 'SAME')
+               or d.get('in_reshape') is not None or d.get('act_nm') in _GN or not plain(d.get('dilation', 1), 1) or not plain(d.get('padding', 'SAME'), 'SAME')
                for d in designs)
 
 
@@ -97,11 +98,19 @@ class _Kernel:
         return [1, src[1], src[2], src[0]]
 
 
+class _GroupNorm:
+    """the variables of one group norm: gamma and beta, no state"""
+
+    def __init__(self, prefix, channels):
+        self.gamma, self.beta, self.channels = prefix + '/GN/gamma', prefix + '/GN/beta', channels
+
+
 class _Net:
     """one net lowered to primitives; owns its variables (flat arenas) and state"""
 
-    def __init__(self, designs, in_ref, name, device, rng, sn_mode, weight_init='default'):
+    def __init__(self, designs, in_ref, name, device, rng, sn_mode, weight_init='default', optimizer='adam'):
         self.name, self.device, self.sn_mode = name, device, sn_mode
+        self.optimizer = optimizer
         self.weight_init = initializers.check_mode(weight_init)          # FLAGS.WEIGHT_INITIALIZER
         # fold a block's 'unpool' x2 / 'avg' /2 into the 3x3 conv next to it (one 4x4 stride-2 launch: 4 taps per pixel
         # instead of 9, no up-sampled tensor in HBM; ResNet-SN config 7.32 -> 6.57 ms per step); MMDGAN_TAPE_COMPOSE=0: two ops
@@ -202,6 +211,17 @@ class _Net:
         self.bns.append((prefix, self.shapes[x][0]))
         return self._emit('bn', [x], self.shapes[x], prefix=prefix, act=act)
 
+    def _norm_act(self, d, scope, suffix, x, act):
+        """the normalisation of `d` with the activation behind it: <scope>/BN<suffix> or <scope>/GN<suffix>"""
+        if d['act_nm'] in _BN:
+            return self._bn_act(scope + '/BN' + suffix, x, act)
+        c, groups = self.shapes[x][0], d['groups']
+        if groups is None:
+            groups = math.gcd(c, 32)
+        if not isinstance(groups, int) or groups < 1 or c % groups:
+            raise ValueError('{}: {} channels do not divide into {} groups'.format(scope, c, groups))
+        return self._emit('gn', [x], self.shapes[x], prefix=scope + '/GN' + suffix, act=act, groups=groups)
+
     def _scale(self, x, scale):                                          # ImageScaling, layer_func.py:1041-1176
         method, factor = scale
         c, h, w = self.shapes[x]
@@ -242,30 +262,30 @@ class _Net:
     def _lower(self, design, x):
         d = dict(_TEMPLATE)
         d.update(design)
-        if d['act_nm'] in ('bn', 'BN') and d['bias'] in ('b', 'bias'):                    # layer_func.py:1241-1242
-            d['bias'] = None
+        if d['act_nm'] in _BN + _GN and d['bias'] in ('b', 'bias'):                       # layer_func.py:1241-1242; a group norm's
+            d['bias'] = None                                                              # beta takes the bias's place as well
         if d['op'] == 'tc':
             d['scale'] = None                                                             # :1245-1247
         scope = '{}/{}'.format(self.name, d['name'])
-        if d['act_nm'] not in (None, 'bn', 'BN'):
+        if d['act_nm'] is not None and d['act_nm'] not in _BN + _GN:
             raise NotImplementedError('{}: {} not implemented'.format(scope, d['act_nm']))
         if d['act'] not in ('linear', 'relu', 'lrelu', 'tanh'):
             raise NotImplementedError('Function {} is not implemented.'.format(d['act']))  # :149
-        bn = d['act_nm'] in ('bn', 'BN')
+        norm = d['act_nm'] is not None
         if d['in_reshape'] is not None:
             x = self._reshape(x, d['in_reshape'])
         if d['type'] in RES_TYPES:
             if d['op'] not in ('c', 'tc'):
                 raise NotImplementedError('{}: residual blocks are built for op "c" and "tc"'.format(scope))
-            y = self._lower_res(d, scope, x, bn)
+            y = self._lower_res(d, scope, x, norm)
         elif d['type'] != 'default':
             raise NotImplementedError('{}: {} is not implemented.'.format(scope, d['type']))   # :2067
         elif d['op'] == 'i':                                             # identity kernel, then BN / activation
-            y = self._bn_act(scope + '/BN', x, d['act']) if bn else self._emit('act', [x], self.shapes[x], act=d['act'])
+            y = self._norm_act(d, scope, '', x, d['act']) if norm else self._emit('act', [x], self.shapes[x], act=d['act'])
         elif d['op'] == 'tc':                                            # transposed conv (layer_func.py:590-600, 918-928)
             y = self._tconv(scope, 'kernel', d, None, x, scope + '/bias/bias' if d['bias'] is not None else None)
-            if bn:
-                y = self._bn_act(scope + '/BN', y, d['act'])
+            if norm:
+                y = self._norm_act(d, scope, '', y, d['act'])
             elif d['act'] != 'linear':
                 y = self._emit('act', [y], self.shapes[y], act=d['act'])
         elif d['op'] in ('d', 'c'):
@@ -280,8 +300,11 @@ class _Net:
                 y = self._emit('dense', [x], [d['out']], k=k)
             else:
                 y = self._conv(scope, 'kernel', d, None, x, bias_name)
-            if bn:
-                y = self._bn_act(scope + '/BN', y, d['act'])
+            if d['op'] == 'd' and d['act_nm'] in _GN and d['out_reshape'] is not None:
+                y = self._reshape(y, d['out_reshape'])                   # groups are of channels: of the image the features become
+                d['out_reshape'] = None
+            if norm:
+                y = self._norm_act(d, scope, '', y, d['act'])
             elif d['act'] != 'linear':
                 y = self._emit('act', [y], self.shapes[y], act=d['act'])
             if d['scale'] is not None and d['scale'][1] < 0:             # :1640-1642
@@ -298,15 +321,15 @@ class _Net:
             'the output shape {} does not match existed shape {}.'.format(self.shapes[x], ref_shape)
         return self._emit('reshape', [x], ref_shape, src_shape=list(self.shapes[x]))
 
-    def _lower_res(self, d, scope, x, bn):                               # layer_func.py:1687-1842
+    def _lower_res(self, d, scope, x, norm):                             # layer_func.py:1687-1842
         act, typ = d['act'], d['type']
         up = d['scale'] is not None and d['scale'][1] > 0
         down = d['scale'] is not None and d['scale'][1] < 0
         bias = d['bias'] is not None
         r = x
         if typ != 'res_v1':
-            if bn:
-                r = self._bn_act(scope + '/BN_0', r, act)
+            if norm:
+                r = self._norm_act(d, scope, '_0', r, act)
             elif act != 'linear':
                 r = self._emit('act', [r], self.shapes[r], act=act)
         # op 'tc' (:1725-1727): kernel_0 and kernel_sc are transposed convs - they ARE the up-sampling, 'scale' was dropped in
@@ -320,8 +343,8 @@ class _Net:
             if up:
                 r = self._scale(r, d['scale'])
             r = self._conv(scope, 'kernel_0', d, 0, r, scope + '/bias_0/bias' if bias else None)
-        if bn:
-            r = self._bn_act(scope + '/BN_1', r, act)
+        if norm:
+            r = self._norm_act(d, scope, '_1', r, act)
         elif act != 'linear':
             r = self._emit('act', [r], self.shapes[r], act=act)
         if down and self._can_fold(d, 1, r, 'avg'):
@@ -390,6 +413,8 @@ class _Net:
                 entries.append((item.w_name, item.kernel_shape))
                 if item.bias_name is not None:
                     entries.append((item.bias_name, [item.out]))
+            elif isinstance(item, _GroupNorm):
+                entries += [(item.gamma, [item.channels]), (item.beta, [item.channels])]
             else:
                 prefix, c = item
                 entries += [(prefix + '/BN/gamma', [c]), (prefix + '/BN/beta', [c])]
@@ -404,7 +429,7 @@ class _Net:
                     z = lambda *shape: torch.zeros(*shape, device=self.device)
                     self.sn[item.scope] = dict(sigma=z(1), scale=z(1), dot=z(1), xbn=z(1), dsigma=z(item.kernel_shape),
                                                u=z(item.sn_u_shape()), un=z(item.sn_u_shape()), xb=z(item.sn_native()))
-            else:
+            elif not isinstance(item, _GroupNorm):
                 prefix, c = item
                 self.state[prefix + '/BN/moving_mean'] = torch.zeros(c, device=self.device)
                 self.state[prefix + '/BN/moving_variance'] = torch.ones(c, device=self.device)
@@ -425,11 +450,30 @@ class _Net:
         moved into its zero-each-step scratch."""
         t = self.opt.step_counter.clone() if hasattr(self, 'opt') else None
         sn_of = {k.w_name: self.sn[k.scope] for k in self.kernels if k.sn}
-        segments = [(off, size, ({q: sn_of[name][q] for q in ('dsigma', 'dot', 'sigma', 'scale')} if name in sn_of else None))
-                    for name, (off, size, _) in self.arena.offsets.items()]
+        fixup = lambda name: {q: sn_of[name][q] for q in ('dsigma', 'dot', 'sigma', 'scale')} if name in sn_of else None
+        # optimizer 'muon': the kernels' updates are orthogonalised (ops.MuonGroup; their momentum lives in the arena of Adam's first
+        # moments), biases and norms' vectors stay with Adam
+        muon = [k.w_name for k in self.kernels] if self.optimizer == 'muon' else []
+        segments = [(off, size, fixup(name)) for name, (off, size, _) in self.arena.offsets.items() if name not in muon]
         self.opt = ops.AdamArena(self.params, self.grads, self.adam_m, self.adam_v, segments)
+        self.muon = None
+        if muon:
+            view = lambda flat: [self.arena.view(name, flat) for name in muon]
+            self.muon = ops.MuonGroup(view(self.params), view(self.grads), view(self.adam_m), fixups=[fixup(name) for name in muon])
         if t is not None:
             self.opt.step_counter.copy_(t)
+
+    def fold_fixup(self, on):
+        """who applies the spectral-norm fix-up: the update as it reads the gradient, or the caller before it"""
+        self.opt.fold_fixup = on
+        if self.muon is not None:
+            self.muon.fold_fixup = on
+
+    def update(self, lr, grad_scale):
+        """the net's parameter update on the current stream"""
+        self.opt.step(lr, grad_scale=grad_scale)
+        if self.muon is not None:
+            self.muon.step(lr, grad_scale=grad_scale)
 
     def effective_grad(self, name):
         """the gradient of variable `name` as the optimiser uses it (native layout, a new tensor): the fix-up applied to
@@ -455,6 +499,8 @@ class _Net:
                 yield p['k']
             elif p['kind'] == 'bn':
                 yield (p['prefix'], self.shapes[p['out']][0])
+            elif p['kind'] == 'gn':
+                yield _GroupNorm(p['prefix'], self.shapes[p['out']][0])
 
     def p(self, name):
         return self.arena.view(name)
@@ -532,6 +578,9 @@ class _Net:
     def init_variables(self, rng):
         """the reference's initialisers (layer_func.py:27-52, 745-747; TF fan rule), reference layouts"""
         for item in self._creation_order():
+            if isinstance(item, _GroupNorm):
+                self.set_variable(item.gamma, np.ones(item.channels, np.float32))
+                continue
             if not isinstance(item, _Kernel):
                 self.set_variable(item[0] + '/BN/gamma', np.ones(item[1], np.float32))
                 continue
@@ -583,8 +632,11 @@ class TapeEngine:
 
     def __init__(self, architecture, loss_type='rep', lr_list=(5e-4, 2e-4), rep_weights=(0.0, -1.0), batch_size=64,
                  seed=0, device=None, dist_group=None, use_graph=False, sn_mode='default', weight_init='default',
-                 mix_threshold=None, launch_mode=None, dp_backend=None):
+                 mix_threshold=None, launch_mode=None, dp_backend=None, optimizer='adam'):
         ops.require_device()
+        if optimizer not in ('adam', 'muon'):
+            raise NotImplementedError('optimizer {} is not implemented.'.format(optimizer))
+        self.optimizer = optimizer
         initializers.check_mode(weight_init)
         if loss_type not in ops.LOSS:
             raise NotImplementedError('Not implemented.')                                # math_func.py:2651
@@ -598,8 +650,8 @@ class TapeEngine:
         self.code_size = architecture['code'][0][0]
         self.in_shape_ref = list(architecture['input'][0])
         rng = np.random.RandomState(seed)
-        self.gen = _Net(architecture['generator'], [self.code_size], 'gen', self.device, rng, sn_mode, weight_init)
-        self.dis = _Net(architecture['discriminator'], self.in_shape_ref, 'dis', self.device, rng, sn_mode, weight_init)
+        self.gen = _Net(architecture['generator'], [self.code_size], 'gen', self.device, rng, sn_mode, weight_init, optimizer)
+        self.dis = _Net(architecture['discriminator'], self.in_shape_ref, 'dis', self.device, rng, sn_mode, weight_init, optimizer)
         assert self.gen.shapes[self.gen.out_val] == self.in_shape_ref, \
             'generator output {} does not match the input shape {}'.format(self.gen.shapes[self.gen.out_val], self.in_shape_ref)
         assert len(self.dis.shapes[self.dis.out_val]) == 1, 'the discriminator must end in a score vector'
@@ -741,7 +793,7 @@ class TapeEngine:
             net.build_optimizer()
             # a single replica folds the spectral-norm fix-up into Adam's read of the gradient; data-parallel replicas apply
             # it before their all-reduce (engine.py: replicas must stay bit-identical)
-            net.opt.fold_fixup = not (self.dist_group is not None and (self.world > 1 or self._dp_force))
+            net.fold_fixup(not (self.dist_group is not None and (self.world > 1 or self._dp_force)))
         self._loss = ops.GanLossLauncher(loss_type, self.rep_weights, self.B, self.score_size, self.device, mix_threshold)
 
     # ---- buffers ----------------------------------------------------------------------------------------------
@@ -753,6 +805,18 @@ class TapeEngine:
         if zero:
             ops.memset_zero(t)                           # (a library call - also on first use: a launch plan records THIS step)
         return t
+
+    def _raw(self, key, nbytes, dtype=torch.uint8):
+        """scratch or statistics of one primitive, at one address for the engine's lifetime (a recorded plan holds it)"""
+        t = self._bufs.get(key)
+        if t is None:
+            t = self._bufs[key] = torch.empty(nbytes // dtype.itemsize, device=self.device, dtype=dtype)
+        assert t.numel() * t.element_size() == nbytes
+        return t
+
+    def _gn_scratch(self, key, n, x_shape, groups):
+        hw = int(np.prod(x_shape[1:-1]))
+        return self._raw(key, int(ops.require_device().mmdgan_gn_workspace_bytes(n, hw, x_shape[-1], groups)))
 
     def _sn_chain_layer(self, net, k):
         """the power iteration of kernel `k` as ops.SnChains describes it (the tensors of _sn_step), or None for a kernel with a
@@ -996,6 +1060,12 @@ class TapeEngine:
                             lib.mmdgan_set_outputs_prezeroed(0)
                 else:
                     ops.bn_fwd_infer(x2, gamma, beta, mm, mv, act=p['act'], out=y2)
+            elif kind == 'gn':                                           # (training and inference are the same)
+                pre, G = p['prefix'], p['groups']
+                y = self._buf_of(key, out_shape)
+                p['_stats'] = self._raw(key + ('stats',), n * G * 16, torch.float64).view(n, G, 2)
+                ops.group_norm_fwd(a, net.p(pre + '/GN/gamma'), net.p(pre + '/GN/beta'), G, act=p['act'], out=y, stats=p['_stats'],
+                                   workspace=self._gn_scratch(key + ('ws',), n, out_shape, G))
             elif kind == 'act':
                 if p['ins'][0] in acted:                                 # written activated by its producer's epilogue
                     y = a
@@ -1028,7 +1098,7 @@ class TapeEngine:
         return vals
 
     # ---- backward ---------------------------------------------------------------------------------------------
-    _ROW_WISE = ('reshape', 'dense', 'conv', 'gconv', 'upconv', 'convdown', 'tconv', 'act', 'down', 'up', 'shuffle', 'add')
+    _ROW_WISE = ('reshape', 'dense', 'conv', 'gconv', 'upconv', 'convdown', 'tconv', 'gn', 'act', 'down', 'up', 'shuffle', 'add')
 
     def _act_fusions(self, net):
         """{value id: activation name} for the values whose ONLY reader is an activation primitive (not the net's output)"""
@@ -1146,7 +1216,7 @@ class TapeEngine:
                 continue
             kind, dy = p['kind'], grads.pop(p['out'])
             vin = p['ins'][0]
-            if vin == 0 and not need_input_grad and kind not in ('dense', 'conv', 'gconv', 'tconv', 'upconv', 'convdown', 'bn'):
+            if vin == 0 and not need_input_grad and kind not in ('dense', 'conv', 'gconv', 'tconv', 'upconv', 'convdown', 'bn', 'gn'):
                 continue
             key = (tag, net.name, i, 'd')
             a = sl(vals[vin])
@@ -1221,6 +1291,16 @@ class TapeEngine:
                 ops.bn_bwd(a.reshape(-1, c), None if resign else y.reshape(-1, c), dy.reshape(-1, c), net.p(pre + '/BN/gamma'), mean,
                            invstd, act=p['act'], dgamma=gg, dbeta=gb, out=dx.view(-1, c), workspace=ws,
                            beta=net.p(pre + '/BN/beta') if resign else None)
+                if param_grads:
+                    self._exchange(net, p)
+                if vin != 0 or need_input_grad:
+                    give(vin, dx)
+            elif kind == 'gn':                                           # (extra rows: the last images' statistics once more)
+                pre, G = p['prefix'], p['groups']
+                dx = self._buf(key, in_shape)
+                ops.group_norm_bwd(a, dy.contiguous(), net.p(pre + '/GN/gamma'), net.p(pre + '/GN/beta'), sl(p['_stats']), act=p['act'], out=dx,
+                                   dgamma=net.g(pre + '/GN/gamma'), dbeta=net.g(pre + '/GN/beta'), param_grads=param_grads,
+                                   workspace=self._gn_scratch(key + ('ws',), in_shape[0], in_shape, G))
                 if param_grads:
                     self._exchange(net, p)
                 if vin != 0 or need_input_grad:
@@ -1377,6 +1457,8 @@ class TapeEngine:
                 names = [p['k'].w_name] + ([p['k'].bias_name] if p['k'].bias_name is not None else [])
             elif p['kind'] == 'bn':
                 names = [p['prefix'] + '/BN/gamma', p['prefix'] + '/BN/beta']
+            elif p['kind'] == 'gn':
+                names = [p['prefix'] + '/GN/gamma', p['prefix'] + '/GN/beta']
             else:
                 continue
             lo = min(net.arena.offsets[n][0] for n in names)
@@ -1505,7 +1587,7 @@ class TapeEngine:
                 # has reached this point; nothing in G's backward pass reads D's weights: D's Adam runs beside it, not at the tail
                 ops.stream_wait(self._wg_raw, main)
                 with torch.cuda.stream(self._wg_stream):
-                    self.dis.opt.step(self.lr_d, grad_scale=1.0)
+                    self.dis.update(self.lr_d, 1.0)
             self._backward(self.gen, gvals, d_in, 'gb', param_grads=True)
             self._wgrad_flush()
             if self._side:
@@ -1520,8 +1602,8 @@ class TapeEngine:
             self._exchange_pending = False
         gs = 1.0 / self.world
         if not d_early:
-            self.dis.opt.step(self.lr_d, grad_scale=gs)
-        self.gen.opt.step(self.lr_g, grad_scale=gs)
+            self.dis.update(self.lr_d, gs)
+        self.gen.update(self.lr_g, gs)
 
     def step(self, real_nhwc=None, z=None, uni=None):
         if z is None:
@@ -1627,9 +1709,11 @@ class TapeEngine:
         """format 2 (GanEngine.state_dict): Adam moments by variable name, independent of the arena layout"""
         m, v, t = self.get_adam_state()
         return {'format': 2, 'global_step': self.global_step, 'variables': self.get_variables(),
-                'loss_state': self._loss.state_dict(), 'adam_m': m, 'adam_v': v, 'adam_t': t}
+                'loss_state': self._loss.state_dict(), 'adam_m': m, 'adam_v': v, 'adam_t': t, 'optimizer': self.optimizer}
 
     def load_state_dict(self, sd):
+        if sd.get('optimizer', 'adam') != self.optimizer:                # (a momentum is no first moment, nor the reverse)
+            raise ValueError('the checkpoint is of optimizer {}, this engine runs {}'.format(sd.get('optimizer', 'adam'), self.optimizer))
         self.set_variables(sd['variables'])
         self.global_step = int(sd['global_step'])
         self._loss.load_state_dict(sd.get('loss_state', {}))

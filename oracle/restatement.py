@@ -47,7 +47,7 @@ def layer_defaults(design):
     """update_layer_design, layer_func.py:1230-1247 (defaults; BN drops the bias)."""
     d = dict(_TEMPLATE)
     d.update(design)
-    if d['act_nm'] in ('bn', 'BN') and d['bias'] in ('b', 'bias'):
+    if d['act_nm'] in ('bn', 'BN', 'gn', 'GN') and d['bias'] in ('b', 'bias'):       # (group norm: as batch norm)
         d['bias'] = None
     if d['op'] == 'tc':
         d['scale'] = None
@@ -210,7 +210,7 @@ def _kernel_spec(layer_scope, op_name, d, index, in_shape, sn_mode, op='c'):
 
 def _build_res(s, d, shape, sn_mode):
     """Layer._add_layer_res_ (layer_func.py:1687-1771)"""
-    sc, bn = s['scope'], d['act_nm'] in ('bn', 'BN')
+    sc, bn = s['scope'], d['act_nm'] in ('bn', 'BN', 'gn', 'GN')
     up = d['scale'] is not None and d['scale'][1] > 0
     down = d['scale'] is not None and d['scale'][1] < 0
     res = {'bn0': bn and d['type'] != 'res_v1', 'bn1': bn, 'up': up, 'down': down,
@@ -378,6 +378,13 @@ def init_params(specs, rng, dtype=torch.float32):
         p[prefix + '/BN/moving_mean'] = torch.zeros(c, dtype=dtype)
         p[prefix + '/BN/moving_variance'] = torch.ones(c, dtype=dtype)
 
+    def norm_vars(d, prefix, c):                              # prefix: <scope>/BN..., a group norm's is <scope>/GN... (no moving statistics)
+        if d['act_nm'] in ('bn', 'BN'):
+            bn_vars(prefix, c)
+        elif d['act_nm'] in ('gn', 'GN'):
+            p[prefix.replace('/BN', '/GN') + '/GN/gamma'] = torch.ones(c, dtype=dtype)
+            p[prefix.replace('/BN', '/GN') + '/GN/beta'] = torch.zeros(c, dtype=dtype)
+
     def kernel_vars(ks, bias_name):
         kd = ks['design']
         p[ks['scope'] + '/kernel'] = torch.as_tensor(init_kernel(rng, ks['kernel_shape'], kd['act']), dtype=dtype)
@@ -391,17 +398,16 @@ def init_params(specs, rng, dtype=torch.float32):
         if 'res' in s:                                                # creation order of layer_func.py:1687-1771
             r = s['res']
             if r['bn0']:
-                bn_vars(sc + '/BN_0', s['in_shape'][0])
+                norm_vars(d, sc + '/BN_0', s['in_shape'][0])
             kernel_vars(r['k0'], sc + '/bias_0/bias' if r['bias'] else None)
             if r['bn1']:
-                bn_vars(sc + '/BN_1', r['k0']['design']['out'])
+                norm_vars(d, sc + '/BN_1', r['k0']['design']['out'])
             kernel_vars(r['k1'], sc + '/bias_1/bias' if r['bias'] else None)
             if 'ksc' in r:
                 kernel_vars(r['ksc'], sc + '/bias_sc/bias')
             continue
         if d['op'] == 'i':
-            if d['act_nm'] in ('bn', 'BN'):
-                bn_vars(sc + '/BN', s['in_shape'][0])
+            norm_vars(d, sc + '/BN', s['in_shape'][0])
             continue
         p[sc + '/kernel/kernel'] = torch.as_tensor(init_kernel(rng, s['kernel_shape'], d['act']), dtype=dtype)
         if d['w_nm'] == 's':                                          # math_func.py:565-567
@@ -414,6 +420,8 @@ def init_params(specs, rng, dtype=torch.float32):
             p[sc + '/BN/BN/beta'] = torch.zeros(c, dtype=dtype)
             p[sc + '/BN/BN/moving_mean'] = torch.zeros(c, dtype=dtype)
             p[sc + '/BN/BN/moving_variance'] = torch.ones(c, dtype=dtype)
+        elif d['act_nm'] in ('gn', 'GN'):
+            norm_vars(d, sc + '/BN', (s['out_shape'] if d['op'] == 'd' else s['op_out_shape'])[0])
     return p
 
 
@@ -538,6 +546,21 @@ def net_forward(specs, params, x, is_training=True, collect=None, masks=None):
             collect.setdefault('pre_acts', []).append(t)
         return _act(t, name, next(mask_iter) if (mask_iter is not None and name in ('relu', 'lrelu')) else None, audit)
 
+    def group_norm(t, prefix, groups):
+        # one image's groups of C / groups channels over all their pixels (biased variance, eps 1e-5); the default is 32 groups or the
+        # largest number below that divides both
+        n, c = t.shape[0], t.shape[1]
+        groups = groups or math.gcd(c, 32)
+        v = t.reshape(n, groups, -1)
+        v = (v - v.mean(dim=2, keepdim=True)) / torch.sqrt(v.var(dim=2, unbiased=False, keepdim=True) + 1e-5)
+        shape = [1, -1] + [1] * (t.dim() - 2)
+        return v.reshape(t.shape) * params[prefix + '/GN/gamma'].reshape(shape) + params[prefix + '/GN/beta'].reshape(shape)
+
+    def norm(t, d, prefix):
+        if d['act_nm'] in ('gn', 'GN'):
+            return group_norm(t, prefix.replace('/BN', '/GN'), d.get('groups'))
+        return batch_norm(t, prefix)
+
     def batch_norm(t, prefix):                                # layer_func.py:953-966, SURVEY A.4
         axis_shape, dims = [1, -1, 1, 1], [0, 2, 3]
         if is_training:
@@ -579,21 +602,21 @@ def net_forward(specs, params, x, is_training=True, collect=None, masks=None):
             '{}: the input shape {} does not match existed shape {}.'.format(sc, list(x.shape[1:]), s['in_shape'])
         if 'res' in s or d['op'] == 'i':
             if d['op'] == 'i':                                # identity kernel, then BN and activation (:1646-1685)
-                if d['act_nm'] in ('bn', 'BN'):
-                    x = batch_norm(x, sc + '/BN')
+                if d['act_nm'] is not None:
+                    x = norm(x, d, sc + '/BN')
                 x = act(x, d['act'])
             else:                                             # Layer._apply_layer_res_, layer_func.py:1773-1842
                 r = s['res']
                 res = x
                 if d['type'] != 'res_v1':
                     if r['bn0']:
-                        res = batch_norm(res, sc + '/BN_0')
+                        res = norm(res, d, sc + '/BN_0')
                     res = act(res, d['act'])
                 if r['up']:
                     res = _rescale(res, d['scale'])
                 res = conv_op(res, r['k0'], sc + '/bias_0/bias' if r['bias'] else None)
                 if r['bn1']:
-                    res = batch_norm(res, sc + '/BN_1')
+                    res = norm(res, d, sc + '/BN_1')
                 res = act(res, d['act'])
                 res = conv_op(res, r['k1'], sc + '/bias_1/bias' if r['bias'] else None)
                 if r['down']:
@@ -649,6 +672,10 @@ def net_forward(specs, params, x, is_training=True, collect=None, masks=None):
                 mean, var = params[sc + '/BN/BN/moving_mean'], params[sc + '/BN/BN/moving_variance']
             x = (x - mean.reshape(axis_shape)) / torch.sqrt(var.reshape(axis_shape) + BN_EPS)
             x = x * params[sc + '/BN/BN/gamma'].reshape(axis_shape) + params[sc + '/BN/BN/beta'].reshape(axis_shape)
+        elif d['act_nm'] in ('gn', 'GN'):
+            if d['op'] == 'd' and d['out_reshape'] is not None:           # groups of channels of the image it becomes
+                x = x.reshape([n] + list(d['out_reshape']))
+            x = group_norm(x, sc + '/GN', d.get('groups'))
         x = act(x, d['act'])
         if d['scale'] is not None and d['scale'][1] < 0:     # layer_func.py:1682-1684
             x = _rescale(x, d['scale'])
