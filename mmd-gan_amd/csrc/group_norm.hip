@@ -56,22 +56,36 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 
 // ---- resident form ----------------------------------------------------------------------------------------------
 // Thread t: float4 column t % CV of the slab, pixels t / CV, t / CV + RT, ...; CV = S / 4 and the thread count are powers of two.
-// red: [row groups][K][CV] doubles, then chan: [2][S] (backward totals of this workgroup), gp / stat: [2][groups' pieces].
-template <int U, bool BWD, bool TANH>
-__global__ __launch_bounds__(kGnMaxThreads) void gn_resident_kernel(GnArgs a) {
+// Per channel the maps are z = A x + B (A = rstd gamma, B = beta - mean A) and dx = A dz + L x + M (L = -rstd^2 m2, M = rstd (rstd mean
+// m2 - m1), per group): three 64-bit multiply-adds and four registers' worth of constants per channel and group.  The backward
+// sums are of dz and dz x, sum dz xhat = rstd (sum dz x - mean sum dz).
+// GP: groups that a thread's four channels can belong to - 1 if D is a multiple of 4 (fewer registers, and the forward sums of the
+// four are one), else 4.  An item of the reduction is a channel, or (forward, GP = 1) a column of four.
+// red: [row groups][NV][CV] doubles, chan: [2][S] (backward totals of this workgroup), stat: [2][S].
+template <int U, bool BWD, bool TANH, int GP>
+__global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= 4 : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
+    constexpr bool kByCol = !BWD && GP == 1;
+    constexpr int NV = kByCol ? 2 : 8;
     extern __shared__ double gn_lds[];
     const int T = blockDim.x, t = threadIdx.x, lane = t & 63;
     const int S = a.S, CV = S >> 2, RT = T / CV, D = a.D, HW = a.HW;
     const int col = t & (CV - 1), row0 = t / CV;
     const int wide = CV < 64 ? 64 : CV, RG = T / wide, rg = t / wide;
-    double *red = gn_lds;                              // backward: [RG][8][CV]; forward: the same layout, 2 * GPT of the 8
-    double *chan = red + RG * 8 * CV;                  // [2][S]
-    double *stat = chan + 2 * S;                       // [2][S]: per group (index = its first item / D)
-    const int slab = blockIdx.x % a.slabs, row = blockIdx.x / a.slabs;
+    double *red = gn_lds;
+    double *chan = red + RG * NV * CV;
+    double *stat = chan + 2 * S;
+    // the slabs of an image share its cache lines: all of them on one XCD (workgroups go to the eight XCDs in turn, each has its
+    // own L2) and close in time - groups of 8 images, image fastest
+    const int group = blockIdx.x / (8 * a.slabs), in = blockIdx.x - group * 8 * a.slabs;
+    const int wide_rows = a.rows - group * 8 < 8 ? a.rows - group * 8 : 8;
+    const int slab = in / wide_rows, row = group * 8 + in % wide_rows;
     const int c0 = slab * S + col * 4, g0 = slab * S / D, gps = S / D;
-    const int DW = D < 64 ? D : 64;                    // adjacent channels that one wave reduces by shuffles
-    float4 gv = *reinterpret_cast<const float4 *>(a.gamma + c0), bv = *reinterpret_cast<const float4 *>(a.beta + c0);
-    const double ga[4] = {gv.x, gv.y, gv.z, gv.w}, be[4] = {bv.x, bv.y, bv.z, bv.w};
+    const int items = kByCol ? CV : S, per_group = kByCol ? D >> 2 : D;      // items, and items per group
+    const int DW = per_group < 64 ? per_group : 64;    // neighbours that one wave reduces by shuffles
+    const int per = per_group / DW;
+    const float4 gv = *reinterpret_cast<const float4 *>(a.gamma + c0), bv = *reinterpret_cast<const float4 *>(a.beta + c0);
+    const float ga[4] = {gv.x, gv.y, gv.z, gv.w}, be[4] = {bv.x, bv.y, bv.z, bv.w};
+    const double inv_m = 1.0 / ((double)HW * D);
     if (BWD && a.part)
         for (int i = t; i < 2 * S; i += T) chan[i] = 0.0;
 
@@ -87,54 +101,60 @@ __global__ __launch_bounds__(kGnMaxThreads) void gn_resident_kernel(GnArgs a) {
             vx[u] = ok ? *reinterpret_cast<const float4 *>(px + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
             if (BWD) vd[u] = ok ? *reinterpret_cast<const float4 *>(pd + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        double mean[4], rstd[4];
-        double s[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] = 0.0;
+        double A[4], B[4], mean[GP], rstd[GP];
         if (BWD) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < GP; ++j) {
                 const double *st = a.stats + 2 * ((size_t)ns * a.G + (c0 + j) / D);
                 mean[j] = st[0]; rstd[j] = st[1];
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { A[j] = rstd[j % GP] * (double)ga[j]; B[j] = fma(-mean[j % GP], A[j], (double)be[j]); }
         }
+        double s[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) s[k] = 0.0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
-            if (!BWD) {
+            float dv[4] = {0.f, 0.f, 0.f, 0.f};
+            if (BWD) { dv[0] = vd[u].x; dv[1] = vd[u].y; dv[2] = vd[u].z; dv[3] = vd[u].w; }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { const double v = xv[j]; s[j] += v; s[4 + j] = fma(v, v, s[4 + j]); }
-            } else {
-                float dv[4] = {vd[u].x, vd[u].y, vd[u].z, vd[u].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {              // (a pixel beyond the image holds dy = 0: it adds nothing)
-                    const double xh = ((double)xv[j] - mean[j]) * rstd[j];
-                    double dz = (double)dv[j] * gn_slope<TANH>(fma(xh, ga[j], be[j]), a.below);
+            for (int j = 0; j < 4; ++j) {
+                const double v = xv[j];
+                if (!BWD) {
+                    s[kByCol ? 0 : j] += v;
+                    s[kByCol ? 1 : 4 + j] = fma(v, v, s[kByCol ? 1 : 4 + j]);
+                } else {                                   // (a pixel beyond the image holds dy = 0: it adds nothing)
+                    double dz = (double)dv[j] * gn_slope<TANH>(fma(A[j], v, B[j]), a.below);
                     if (TANH) { dv[j] = (float)dz; dz = (double)dv[j]; }      // evaluated once: dz itself, in 32 bits, for the second pass
                     s[j] += dz;
-                    s[4 + j] = fma(dz, xh, s[4 + j]);
+                    s[(4 + j) % NV] = fma(dz, v, s[(4 + j) % NV]);
                 }
-                if (TANH) vd[u] = make_float4(dv[0], dv[1], dv[2], dv[3]);
             }
+            if (BWD && TANH) vd[u] = make_float4(dv[0], dv[1], dv[2], dv[3]);
         }
         // lanes of a wave that hold the same column
         for (int o = 32; o >= CV; o >>= 1) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] += __shfl_xor(s[k], o, 64);
+            for (int k = 0; k < NV; ++k) s[k] += __shfl_xor(s[k], o, 64);
         }
         if (CV >= 64 || lane < CV) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) red[(rg * 8 + k) * CV + col] = s[k];
+            for (int k = 0; k < NV; ++k) red[(rg * NV + k) * CV + col] = s[k];
         }
         __syncthreads();
-        // item = channel of the slab: totals over the row groups, then over the group's channels
-        for (int i = t; i < S; i += T) {
+        // totals over the row groups, then over the group's items
+        for (int i = t; i < items; i += T) {
+            const int k = kByCol ? 0 : i & 3, q = kByCol ? i : i >> 2;
             double s1 = 0.0, s2 = 0.0;
-            for (int q = 0; q < RG; ++q) {
-                s1 += red[(q * 8 + (i & 3)) * CV + (i >> 2)];
-                s2 += red[(q * 8 + 4 + (i & 3)) * CV + (i >> 2)];
+            for (int z = 0; z < RG; ++z) {
+                s1 += red[(z * NV + k) * CV + q];
+                s2 += red[(z * NV + (kByCol ? 1 : 4) + k) * CV + q];
             }
             if (BWD) {
+                const double *st = a.stats + 2 * ((size_t)ns * a.G + (slab * S + i) / D);
+                s2 = st[1] * fma(-st[0], s1, s2);
                 if (a.part && n < a.x_batch) { chan[i] += s1; chan[S + i] += s2; }
                 const double g = (double)a.gamma[slab * S + i];
                 s1 *= g; s2 *= g;
@@ -143,31 +163,34 @@ __global__ __launch_bounds__(kGnMaxThreads) void gn_resident_kernel(GnArgs a) {
             if ((i & (DW - 1)) == 0) { stat[i / DW] = s1; stat[S + i / DW] = s2; }
         }
         __syncthreads();
-        const double inv_m = 1.0 / ((double)HW * D);
-        const int per = D / DW;
-        double m1[4], m2[4];
+        double L[GP], M[GP];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < GP; ++j) {
             const int g = (col * 4 + j) / D;
             double s1 = 0.0, s2 = 0.0;
             for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
-            m1[j] = s1 * inv_m; m2[j] = s2 * inv_m;
-            if (!BWD) {
-                mean[j] = m1[j];
-                double var = m2[j] - m1[j] * m1[j];
+            s1 *= inv_m; s2 *= inv_m;
+            if (BWD) {
+                L[j] = -rstd[j] * rstd[j] * s2;
+                M[j] = -fma(L[j], mean[j], rstd[j] * s1);
+            } else {
+                double var = fma(-s1, s1, s2);
                 if (var < 0.0) var = 0.0;
-                rstd[j] = 1.0 / sqrt(var + (double)a.eps);
+                mean[j] = s1; rstd[j] = 1.0 / sqrt(var + (double)a.eps);
             }
         }
         if (!BWD) {
-            for (int g = t; g < gps; g += T) {
-                double s1 = 0.0, s2 = 0.0;
-                for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
-                const double mu = s1 * inv_m;
-                double var = s2 * inv_m - mu * mu;
-                if (var < 0.0) var = 0.0;
-                double *st = a.stats + 2 * ((size_t)n * a.G + g0 + g);
-                st[0] = mu; st[1] = 1.0 / sqrt(var + (double)a.eps);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { A[j] = rstd[j % GP] * (double)ga[j]; B[j] = fma(-mean[j % GP], A[j], (double)be[j]); }
+            // one thread per group publishes what its own channels use
+            if (row0 == 0) {
+#pragma unroll
+                for (int j = 0; j < GP; ++j) {
+                    if ((col * 4 + j) % D == 0) {
+                        double *st = a.stats + 2 * ((size_t)n * a.G + g0 + (col * 4 + j) / D);
+                        st[0] = mean[j]; st[1] = rstd[j];
+                    }
+                }
             }
         }
         float *po = a.out + (size_t)n * HW * a.C + c0;
@@ -177,22 +200,17 @@ __global__ __launch_bounds__(kGnMaxThreads) void gn_resident_kernel(GnArgs a) {
             gn_fresh(vx[u]);
             if (BWD) gn_fresh(vd[BWD ? u : 0]);
             const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
-            float o[4];
-            if (!BWD) {
+            float dv[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+            if (BWD) { dv[0] = vd[u].x; dv[1] = vd[u].y; dv[2] = vd[u].z; dv[3] = vd[u].w; }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = gn_act<TANH>((float)fma(((double)xv[j] - mean[j]) * rstd[j], ga[j], be[j]), a.below);
-            } else {
-                const float dv[4] = {vd[u].x, vd[u].y, vd[u].z, vd[u].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double xh = ((double)xv[j] - mean[j]) * rstd[j];
-                    const double dz = TANH ? (double)dv[j] : (double)dv[j] * gn_slope<false>(fma(xh, ga[j], be[j]), a.below);
-                    o[j] = (float)(rstd[j] * (fma(ga[j], dz, -m1[j]) - xh * m2[j]));
-                }
+            for (int j = 0; j < 4; ++j) {
+                const double v = xv[j], z = fma(A[j], v, B[j]);
+                if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
+                else o[j] = (float)fma(A[j], TANH ? (double)dv[j] : (double)dv[j] * gn_slope<false>(z, a.below), fma(L[j % GP], v, M[j % GP]));
             }
             if (r < HW) *reinterpret_cast<float4 *>(po + (size_t)r * a.C) = make_float4(o[0], o[1], o[2], o[3]);
         }
-        __syncthreads();                               // red and stat are written again for the next image
+        if (n + a.rows < a.N) __syncthreads();         // red and stat are written again for the next image
     }
     if (BWD && a.part) {
         for (int i = t; i < S; i += T) {               // (the thread that owns item i wrote chan[i])
@@ -220,6 +238,12 @@ __device__ __forceinline__ GnSlab gn_slab(const GnArgs &a, int s) {
     return r;
 }
 
+// lanes of a 256-thread workgroup that add up one of `groups` (at most 256) groups: a power of two up to a wave
+__device__ __forceinline__ int gn_lanes(int groups) {
+    int l = 64;
+    while (l > 1 && groups * l > 256) l >>= 1;
+    return l;
+}
 template <int VEC> __device__ __forceinline__ void gn_load(const float *p, float *v) {
     if (VEC == 4) {
         const float4 q = *reinterpret_cast<const float4 *>(p);
@@ -304,23 +328,14 @@ __global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
     __syncthreads();
     const int P = a.chunks * a.pieces, p = chunk * a.pieces + sl.piece;
     const int per = sl.groups == 1 ? sl.width : a.D;   // channels of a group in this slab
-    if (per <= 8) {
-        for (int g = t; g < sl.groups; g += 256) {
-            double u1 = 0.0, u2 = 0.0;
-            for (int q = 0; q < per; ++q) { u1 += chan[0][g * per + q]; u2 += chan[1][g * per + q]; }
-            double *o = a.gpart + (((size_t)n * a.G + sl.g0 + g) * P + p) * 2;
-            o[0] = u1; o[1] = u2;
-        }
-    } else {
-        for (int g = t >> 6; g < sl.groups; g += 4) {
-            double u1 = 0.0, u2 = 0.0;
-            for (int q = t & 63; q < per; q += 64) { u1 += chan[0][g * per + q]; u2 += chan[1][g * per + q]; }
-            u1 = wave_sum(u1); u2 = wave_sum(u2);
-            if ((t & 63) == 0) {
-                double *o = a.gpart + (((size_t)n * a.G + sl.g0 + g) * P + p) * 2;
-                o[0] = u1; o[1] = u2;
-            }
-        }
+    const int lanes = gn_lanes(sl.groups), g = t / lanes, l = t & (lanes - 1);
+    double u1 = 0.0, u2 = 0.0;
+    if (g < sl.groups)
+        for (int q = l; q < per; q += lanes) { u1 += chan[0][g * per + q]; u2 += chan[1][g * per + q]; }
+    for (int o = lanes >> 1; o > 0; o >>= 1) { u1 += __shfl_xor(u1, o, 64); u2 += __shfl_xor(u2, o, 64); }
+    if (g < sl.groups && l == 0) {
+        double *o = a.gpart + (((size_t)n * a.G + sl.g0 + g) * P + p) * 2;
+        o[0] = u1; o[1] = u2;
     }
 }
 
@@ -348,22 +363,15 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
             st[0] = mu; st[1] = is;
         }
     };
-    if (P <= 8) {
-        for (int g = t; g < sl.groups; g += 256) {
-            const double *q = a.gpart + ((size_t)n * a.G + sl.g0 + g) * P * 2;
-            double u1 = 0.0, u2 = 0.0;
-            for (int p = 0; p < P; ++p) { u1 += q[2 * p]; u2 += q[2 * p + 1]; }
-            publish(g, u1, u2);
-        }
-    } else {
-        for (int g = t >> 6; g < sl.groups; g += 4) {
-            const double *q = a.gpart + ((size_t)n * a.G + sl.g0 + g) * P * 2;
-            double u1 = 0.0, u2 = 0.0;
-            for (int p = t & 63; p < P; p += 64) { u1 += q[2 * p]; u2 += q[2 * p + 1]; }
-            u1 = wave_sum(u1); u2 = wave_sum(u2);
-            if ((t & 63) == 0) publish(g, u1, u2);
-        }
+    const int lanes = gn_lanes(sl.groups), mine = t / lanes, l = t & (lanes - 1);
+    double u1 = 0.0, u2 = 0.0;
+    if (mine < sl.groups) {
+        const double2 *q = reinterpret_cast<const double2 *>(a.gpart + ((size_t)n * a.G + sl.g0 + mine) * P * 2);
+#pragma unroll 4
+        for (int p = l; p < P; p += lanes) { const double2 v = q[p]; u1 += v.x; u2 += v.y; }
     }
+    for (int o = lanes >> 1; o > 0; o >>= 1) { u1 += __shfl_xor(u1, o, 64); u2 += __shfl_xor(u2, o, 64); }
+    if (mine < sl.groups && l == 0) publish(mine, u1, u2);
     __syncthreads();
     if (rl >= RT) return;
     const int c = sl.c0 + col * VEC;
@@ -452,11 +460,11 @@ static void gn_plan_resident(long HW, int C, int D, long N, bool bwd, GnPlan &p)
     if (top < D) return;
     const long cap = (long)kGnMaxThreads * (bwd ? kGnBwdRegs : kGnFwdRegs);      // float4 per tensor
     int least = D < 4 ? 4 : D;
-    // a slab of 64 channels where there are workgroups enough with it, down to 16 (64 bytes a pixel) where there are not or
-    // where the image needs it
+    // a slab of 64 channels, down to 8 where it takes that to occupy the CUs or to hold the image (32x64x64x64 forward 28.1 us on
+    // 16 channels and half of the CUs, 19.5 on 8; with 256 workgroups already, 64x32x32x64 takes 11.1 on 16 and 12.9 on 8)
     int S = top < 64 ? top : 64;
     if (S < least) S = least;
-    while (S > least && S > 16 && (N * (C / S) < 256 || HW * (S / 4) > cap)) S >>= 1;
+    while (S > least && S > 8 && (N * (C / S) < 256 || HW * (S / 4) > cap)) S >>= 1;
     if (HW * (S / 4) > cap) return;
     const long total = HW * (S / 4);
     long T = 64;
@@ -493,18 +501,18 @@ static size_t gn_bytes(long N, long HW, int C, int G) {
 
 static bool gn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-template <bool BWD, bool TANH>
+template <bool BWD, bool TANH, int GP>
 static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st) {
     const int CV = p.S / 4, wide = CV < 64 ? 64 : CV;
-    const size_t lds = ((size_t)(p.T / wide) * 8 * CV + 4 * (size_t)p.S) * sizeof(double);
+    const size_t lds = ((size_t)(p.T / wide) * (!BWD && GP == 1 ? 2 : 8) * CV + 4 * (size_t)p.S) * sizeof(double);
     const dim3 grid((unsigned)(a.rows * a.slabs)), block(p.T);
     switch (p.U) {
-        case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH>), grid, block, lds, st, a); break;
-        case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH>), grid, block, lds, st, a); break;
-        case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH>), grid, block, lds, st, a); break;
-        case 8: hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH>), grid, block, lds, st, a); break;
-        case 16: hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH>), grid, block, lds, st, a); break;
-        default: hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH>), grid, block, lds, st, a); break;   // forward only (plan)
+        case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        case 8: hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        case 16: hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        default: hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH, GP>), grid, block, lds, st, a); break;   // forward only (plan)
     }
 }
 
@@ -521,7 +529,8 @@ static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipSt
         a.rows = (int)gn_resident_rows(a.N, a.slabs);
         part_rows = a.rows;
         a.part = params ? (double *)workspace : nullptr;
-        gn_launch_resident<BWD, TANH>(a, p, st);
+        if (a.D % 4 == 0) gn_launch_resident<BWD, TANH, 1>(a, p, st);
+        else gn_launch_resident<BWD, TANH, 4>(a, p, st);
     } else {
         gn_plan_split(a.HW, a.C, a.D, a.N, p);
         a.SB = p.SB; a.gps = p.gps; a.pieces = p.pieces; a.slabs = p.slabs; a.chunks = p.chunks; a.chunk_px = p.chunk_px;
@@ -555,6 +564,7 @@ using namespace mmdgan;
     MMDGAN_REQUIRE(N >= 1 && HW >= 1 && C >= 1 && G >= 1, what ": bad size N=%d HW=%ld C=%d G=%d", N, HW, C, G);                      \
     MMDGAN_REQUIRE(C % G == 0, what ": %d channels do not divide into %d groups", C, G);                                              \
     MMDGAN_REQUIRE(N <= 65535 && HW <= 0x7fffffffL / C, what ": image of %ld pixels x %d channels or batch of %d is too large", HW, C, N); \
+    MMDGAN_REQUIRE(!((uintptr_t)workspace & 15), what ": the workspace is not 16-byte aligned");                                       \
     MMDGAN_REQUIRE(act >= MMDGAN_ACT_LINEAR && act <= MMDGAN_ACT_TANH, what ": unknown activation %d", act)
 
 extern "C" size_t mmdgan_gn_workspace_bytes(int N, long HW, int C, int G) {

@@ -19,7 +19,7 @@ def test_group_norm_refuses_bad_geometries(lib):
     for kw, word in ((dict(N=0), 'bad size'), (dict(HW=0), 'bad size'), (dict(C=0), 'bad size'), (dict(G=0), 'bad size'),
                      (dict(G=-1), 'bad size'), (dict(G=5), 'do not divide'), (dict(G=24), 'do not divide'), (dict(act=4), 'activation'),
                      (dict(act=-1), 'activation'), (dict(eps=0.0), 'eps'), (dict(N=65536), 'too large'), (dict(HW=1 << 30), 'too large'),
-                     (dict(x=None), 'null'), (dict(stats=None), 'null'), (dict(ws=None), 'null')):
+                     (dict(ws=24), 'aligned'), (dict(x=None), 'null'), (dict(stats=None), 'null'), (dict(ws=None), 'null')):
         assert fwd(**kw) == -1, kw
         assert word in message(lib), (kw, message(lib))
 
