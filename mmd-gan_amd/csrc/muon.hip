@@ -61,19 +61,19 @@ __device__ __forceinline__ void mu_put8(f16 *o, size_t at, const float (&v)[8]) 
 constexpr int kMuStage = 8 * 4096;                           // bytes of a stage: four row blocks of a, four of b
 __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, size_t sb, int steps, char *lds, f32x16 (&acc)[2][2]) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    struct Set { mu_u32x4 a[4], b[4]; } r0, r1;
-    auto fetch = [&](int s, Set &x) {
+    mu_u32x4 ga[4], gb[4];
+    auto fetch = [&](int s) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x.a[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
-            x.b[i] = *reinterpret_cast<const mu_u32x4 *>(b + i * sb + (size_t)s * 2048 + t * 8);
+            ga[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
+            gb[i] = *reinterpret_cast<const mu_u32x4 *>(b + i * sb + (size_t)s * 2048 + t * 8);
         }
     };
-    auto store = [&](char *buf, const Set &x) {
+    auto store = [&](char *buf) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<mu_u32x4 *>(buf + i * 4096 + t * 16) = x.a[i];
-            *reinterpret_cast<mu_u32x4 *>(buf + (4 + i) * 4096 + t * 16) = x.b[i];
+            *reinterpret_cast<mu_u32x4 *>(buf + i * 4096 + t * 16) = ga[i];
+            *reinterpret_cast<mu_u32x4 *>(buf + (4 + i) * 4096 + t * 16) = gb[i];
         }
     };
     f32x16 low[2][2];                                        // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
@@ -82,44 +82,50 @@ __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, s
 #pragma unroll
         for (int j = 0; j < 2; ++j) { acc[i][j] = f32x16{}; low[i][j] = f32x16{}; }
     const int ar = (w >> 1) * 2 * 4096 + lane * 16, br = (4 + (w & 1) * 2) * 4096 + lane * 16;
-    auto multiply = [&](const char *buf) {
+    struct Frag { f16x8 ah[2], al[2], bh[2], bl[2]; } f0, f1;
+    auto read = [&](Frag &f, const char *buf, int ks) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            f16x8 ah[2], al[2], bh[2], bl[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                ah[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048);
-                al[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048 + 1024);
-                bh[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048);
-                bl[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048 + 1024);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
-                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
-                }
+        for (int i = 0; i < 2; ++i) {
+            f.ah[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048);
+            f.al[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048 + 1024);
+            f.bh[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048);
+            f.bl[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048 + 1024);
         }
     };
-    // loads run two stages ahead of the products (one stage is 768 MFMA cycles, a miss takes longer); the barriers publish LDS
-    // only and leave them in flight.  `steps` is even.
-    fetch(0, r0);
-    fetch(1, r1);
-    store(lds, r0);
+    auto multiply = [&](const Frag &f) {                     // (an accumulator is touched every fourth product)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], low[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], low[i][j], 0, 0, 0);
+    };
+    // Everything that a group of products needs was asked for one group earlier: operands of the second half of a stage are read from
+    // LDS under the products of the first, those of the next stage's first half under the products of the second; global loads
+    // run a stage and a half ahead.  The barrier publishes LDS only and leaves them in flight.
+    fetch(0);
+    store(lds);
+    fetch(1);                                                // (steps >= 2)
     lds_barrier();
-    for (int s = 0; s < steps; s += 2) {
-        const bool more = s + 2 < steps;
-        if (more) fetch(s + 2, r0);
-        multiply(lds);
-        store(lds + kMuStage, r1);
+    read(f0, lds, 0);
+    for (int s = 0; s < steps; ++s) {
+        char *cur = lds + (s & 1) * kMuStage, *nxt = lds + ((s + 1) & 1) * kMuStage;
+        const bool more = s + 1 < steps;
+        read(f1, cur, 1);
+        multiply(f0);
+        if (more) store(nxt);                                // (every wave has read the stage before last: the barrier below)
         lds_barrier();
-        if (more) fetch(s + 3, r1);
-        multiply(lds + kMuStage);
-        if (more) store(lds, r0);
-        lds_barrier();
+        if (more) read(f0, nxt, 0);
+        if (s + 2 < steps) fetch(s + 2);
+        multiply(f1);
     }
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -361,7 +367,7 @@ __global__ __launch_bounds__(256) void mu_gram_reduce_kernel(MuGramTable t) {
     }
 }
 
-// ---- m x m products of commuting symmetric matrices: one triangle of 64 x 64 tiles --------------------------------
+// ---- m x m products of commuting symmetric matrices: one triangle of tiles --------------------------------
 struct MuSquare {
     const f16 *a, *b;                // o = alpha a b  (packed, symmetric, [mp, mp])
     f16 *o;
@@ -371,111 +377,91 @@ struct MuSquare {
 };
 struct MuSquareTable { MuFirst<2 * kMuGroup> f; MuSquare j[2 * kMuGroup]; };
 
-// Latency-bound (one matrix has 36 tiles at m = 512): no staging, the four waves of a tile take the 32-wide reduction steps in turn,
-// each straight from L2 into MFMA operands with the next step's loads in flight, and their sums meet in LDS.
+// Latency-bound: no staging, tiles of 32 x 32 (136 workgroups from one matrix of m = 512), the four waves of a tile take the 32-wide
+// reduction steps in turn, each straight from L2 into MFMA operands with kMuAhead steps in flight, and their sums meet in LDS.
+// A launch at m = 512 takes 5.9 us (64 x 64 tiles on 36 workgroups: 9.8).  At m = 1024 the finer tiles read twice as much from L2 and
+// still win, several workgroups to a CU covering each other's waits: the whole update of the 64 x 64 images' discriminator takes 1.02 ms,
+// with 64 x 64 tiles above m = 512 it took 1.11.
+constexpr int kMuAhead = 2;
+
+// tile number -> (ti, tj), ti >= tj, of a triangle of nb rows: in blocks of 4 x 4 tiles where nb allows, so that an XCD's run of
+// neighbours needs few row blocks (that update without it: 1.04 ms)
+__device__ __forceinline__ void mu_tri_blocked(int t, int nb, int &ti, int &tj) {
+    if (nb & 3) { mu_tri(t, ti, tj); return; }
+    int si = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.125f);        // 8 si^2 + 2 si tiles before block row si
+    while (8 * (si + 1) * (si + 1) + 2 * (si + 1) <= t) ++si;
+    while (8 * si * si + 2 * si > t) --si;
+    t -= 8 * si * si + 2 * si;
+    if (t < 16 * si) { ti = si * 4 + ((t >> 2) & 3); tj = (t >> 4) * 4 + (t & 3); return; }
+    mu_tri(t - 16 * si, ti, tj);
+    ti += si * 4; tj += si * 4;
+}
+// a 32 x 32 sum in LDS, eight-column groups of row r at group ^ (r & 3)
+__device__ __forceinline__ int mu_lds32(int r, int c) { return r * 32 + (((c >> 3) ^ (r & 3)) << 3) + (c & 7); }
+
 __global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
-    __shared__ __attribute__((aligned(16))) float part[4][64 * 64];
+    __shared__ __attribute__((aligned(16))) float part[4][32 * 32];
     const int q = mu_which(t.f, blockIdx.x);
     const MuSquare &p = t.j[q];
-    int ti, tj;
     const int item = mu_item(blockIdx.x - t.f.first[q], p.tiles);
     if (item < 0) return;
-    mu_tri(item, ti, tj);
+    int ti, tj;
+    mu_tri_blocked(item, p.mp / 32, ti, tj);
     const int kb = p.mp / 16, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const size_t sr = mu_strip(kb);
-    const f16 *a = p.a + (size_t)ti * 2 * sr + lane * 8, *b = p.b + (size_t)tj * 2 * sr + lane * 8;
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-    f16x8 fa[2][2][2], fb[2][2][2];                          // [ks][block][hi, lo]
-    auto fetch = [&](int s, f16x8 (&xa)[2][2][2], f16x8 (&xb)[2][2][2]) {
+    const f16 *a = p.a + ti * sr + lane * 8, *b = p.b + tj * sr + lane * 8;
+    struct Step { f16x8 a[2][2], b[2][2]; } f[kMuAhead];     // [ks][hi, lo]
+    auto fetch = [&](int s, Step &x) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    xa[ks][i][h] = *reinterpret_cast<const f16x8 *>(a + i * sr + (size_t)s * 2048 + ks * 1024 + h * 512);
-                    xb[ks][i][h] = *reinterpret_cast<const f16x8 *>(b + i * sr + (size_t)s * 2048 + ks * 1024 + h * 512);
-                }
+            for (int h = 0; h < 2; ++h) {
+                x.a[ks][h] = *reinterpret_cast<const f16x8 *>(a + (size_t)s * 2048 + ks * 1024 + h * 512);
+                x.b[ks][h] = *reinterpret_cast<const f16x8 *>(b + (size_t)s * 2048 + ks * 1024 + h * 512);
+            }
     };
-    auto multiply = [&](const f16x8 (&xa)[2][2][2], const f16x8 (&xb)[2][2][2]) {
+    const int steps = p.mp / 128;                            // of this wave: w, w + 4, ...
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+    for (int i = 0; i < kMuAhead; ++i)
+        if (i < steps) fetch(w + 4 * i, f[i]);
+    // the result goes out in pieces of 8 values of a row, 64 to a block of 32 rows and 16 columns in lane order: waves 0 and 1 write the
+    // tile, waves 2 and 3 its mirror image.  Their pieces of z are asked for with the operands.
+    const bool mirror = w >= 2;
+    const int r = lane & 31, k = (w & 1) * 16 + (lane >> 5) * 8, R = (mirror ? tj : ti) * 32 + r, K = (mirror ? ti : tj) * 32 + k;
+    const size_t o = mu_off(R, K, kb);
+    f16x8 zh, zl;
+    if (p.z) { zh = *reinterpret_cast<const f16x8 *>(p.z + o); zl = *reinterpret_cast<const f16x8 *>(p.z + o + 512); }
+    f32x16 acc = {}, low = {};
+    for (int s0 = 0; s0 < steps; s0 += kMuAhead) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kMuAhead; ++i) {
+            if (s0 + i < steps) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][0], xb[ks][j][1], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][1], xb[ks][j][0], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[ks][i][0], xb[ks][j][0], acc[i][j], 0, 0, 0);
+                for (int ks = 0; ks < 2; ++ks) {
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i].a[ks][0], f[i].b[ks][0], acc, 0, 0, 0);
+                    low = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i].a[ks][0], f[i].b[ks][1], low, 0, 0, 0);
+                    low = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i].a[ks][1], f[i].b[ks][0], low, 0, 0, 0);
                 }
-    };
-    const int steps = p.mp / 32;                             // a multiple of 4: every wave has the same number
-    fetch(w, fa, fb);
-    // 512 pieces of 8 values of a row: block (row block, 16 columns) = w * 2 + i
-    f16x8 zh[2], zl[2];
-    if (p.z) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int blk = w * 2 + i;
-            const size_t o = mu_off(ti * 64 + (blk >> 2) * 32 + (lane & 31), tj * 64 + (blk & 3) * 16 + (lane >> 5) * 8, kb);
-            zh[i] = *reinterpret_cast<const f16x8 *>(p.z + o); zl[i] = *reinterpret_cast<const f16x8 *>(p.z + o + 512);
-        }
-    }
-    for (int s = w; s < steps; s += 4) {
-        f16x8 na[2][2][2], nb[2][2][2];
-        const bool more = s + 4 < steps;
-        if (more) fetch(s + 4, na, nb);
-        multiply(fa, fb);
-        if (more) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) { fa[ks][i][h] = na[ks][i][h]; fb[ks][i][h] = nb[ks][i][h]; }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) part[w][mu_lds(i * 32 + mu_row(e), j * 32 + mu_col())] = acc[i][j][e];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int blk = w * 2 + i, r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
-        const int at = mu_lds(r, k);
-        const size_t o = mu_off(ti * 64 + r, tj * 64 + k, kb);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = p.alpha * ((part[0][at + e] + part[1][at + e]) + (part[2][at + e] + part[3][at + e]));
-            if (p.z) {
-                v[e] += p.zscale * ((float)zh[i][e] + (float)zl[i][e]);
-                if (ti * 64 + r == tj * 64 + k + e) v[e] += p.diag;
+                if (s0 + i + kMuAhead < steps) fetch(w + 4 * (s0 + i + kMuAhead), f[i]);
             }
         }
-        mu_put8(p.o, o, v);
-        if (ti != tj) {
+    }
+    acc += low;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[0][at + e] = v[e];          // (this thread's own piece: nobody else reads it before the barrier)
+    for (int e = 0; e < 16; ++e) part[w][mu_lds32(mu_row(e), mu_col())] = acc[e];
+    __syncthreads();
+    if (mirror && ti == tj) return;                          // (a tile on the diagonal holds both halves)
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int at = mirror ? mu_lds32(k + e, r) : mu_lds32(r, k) + e;
+        v[e] = p.alpha * ((part[0][at] + part[1][at]) + (part[2][at] + part[3][at]));
+        if (p.z) {
+            v[e] += p.zscale * ((float)zh[e] + (float)zl[e]);
+            if (R == K + e) v[e] += p.diag;
         }
     }
-    if (ti == tj) return;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int blk = w * 2 + i, c = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = part[0][mu_lds(k + e, c)];
-        mu_put8(p.o, mu_off(tj * 64 + c, ti * 64 + k, kb), v);
-    }
+    mu_put8(p.o, o, v);
 }
 
 // ---- X <- P X, between two chains (packed, both layouts) or as the result ------------------------------------------
@@ -674,7 +660,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
                 p = MuSquare{};
                 p.a = (const f16 *)(ws + a); p.b = (const f16 *)(ws + b); p.o = (f16 *)(ws + o); p.alpha = alpha;
                 p.mp = m[i].mp;
-                const int tb = p.mp / 64;
+                const int tb = p.mp / 32;
                 p.tiles = tb * (tb + 1) / 2;
                 t.f.first[nt++] = blocks;
                 blocks += (p.tiles + 7) & ~7;
