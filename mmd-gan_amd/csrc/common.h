@@ -74,6 +74,11 @@ inline int check_launch(const char *what) {
         }                                    \
     } while (0)
 
+// whether two device arrays share a byte
+inline bool spans_meet(const void *a, size_t na, const void *b, size_t nb) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 // forward activation (layer_func.py:104-151)
 __device__ __forceinline__ float act_fwd(float v, int act) {
     switch (act) {

@@ -9,7 +9,7 @@
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.  What the kernels do about it:
 //   gn_resident   one workgroup holds an image's channel slab (whole groups, all pixels) in registers between the sums and
 //                 the apply, so every tensor moves once.  Needs D a power of two and a slab of at most 256 KB (forward) /
-//                 128 KB per tensor (backward).
+//                 128 KB per tensor (backward; with tanh 64 KB).
 //   gn_partial + gn_apply   everything else: pixel chunks' sums to the workspace, then the apply pass reads x (and dy) again.
 // All arithmetic on elements is in 64 bits: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for memory
 // either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
@@ -19,7 +19,10 @@
 namespace mmdgan {
 
 constexpr int kGnMaxThreads = 512;                   // 256 VGPRs per wave: at most half of them hold the slab
-constexpr int kGnFwdRegs = 32, kGnBwdRegs = 16;      // float4 per thread and tensor
+// float4 per thread and tensor; tanh's code costs registers that a backward with 16 does not have (its spills made 32x64x64x64
+// 78 us, in two passes it takes 48; and 64x8x8x512 23 us where half of the registers had to do, now 13)
+constexpr int kGnFwdRegs = 32;
+template <bool TANH> constexpr int kGnBwdRegs = TANH ? 8 : 16;
 constexpr int kGnGrid = 1024;                        // workgroups of a launch: four per CU
 constexpr int kGnSplitCh = 256;                      // channels of a slab in the two-pass form
 
@@ -63,7 +66,7 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 // four are one), else 4.  An item of the reduction is a channel, or (forward, GP = 1) a column of four.
 // red: [row groups][NV][CV] doubles, chan: [2][S] (backward totals of this workgroup), stat: [2][S].
 template <int U, bool BWD, bool TANH, int GP>
-__global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= 4 : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
+__global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
     constexpr bool kByCol = !BWD && GP == 1;
     constexpr int NV = kByCol ? 2 : 8;
     extern __shared__ double gn_lds[];
@@ -452,13 +455,14 @@ struct GnPlan {
     int S, T, U;                 // resident: slab channels, threads, float4 per thread
     int SB, gps, pieces, slabs, chunks, chunk_px;     // two-pass
 };
-static void gn_plan_resident(long HW, int C, int D, long N, bool bwd, GnPlan &p) {
+// regs: float4 per thread and tensor at most
+static void gn_plan_resident(long HW, int C, int D, long N, int regs, GnPlan &p) {
     p.resident = false;
     if ((C & 3) || !gn_pow2(D) || D > kGnSplitCh) return;
     int top = 4;                                       // widest power-of-two slab that divides C
     while (top < kGnSplitCh && C % (top * 2) == 0) top *= 2;
     if (top < D) return;
-    const long cap = (long)kGnMaxThreads * (bwd ? kGnBwdRegs : kGnFwdRegs);      // float4 per tensor
+    const long cap = (long)kGnMaxThreads * regs;
     int least = D < 4 ? 4 : D;
     // a slab of 64 channels, down to 8 where it takes that to occupy the CUs or to hold the image (32x64x64x64 forward 28.1 us on
     // 16 channels and half of the CUs, 19.5 on 8; with 256 workgroups already, 64x32x32x64 takes 11.1 on 16 and 12.9 on 8)
@@ -511,15 +515,15 @@ static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st)
         case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH, GP>), grid, block, lds, st, a); break;
         case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH, GP>), grid, block, lds, st, a); break;
         case 8: hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case 16: hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        default: hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH, GP>), grid, block, lds, st, a); break;   // forward only (plan)
+        case 16: if constexpr (!BWD || kGnBwdRegs<TANH> == 16) hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH, GP>), grid, block, lds, st, a); break;
+        case kGnFwdRegs: if constexpr (!BWD) hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH, GP>), grid, block, lds, st, a); break;
     }
 }
 
 template <bool BWD, bool TANH>
 static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipStream_t st, const char *what) {
     GnPlan p;
-    gn_plan_resident(a.HW, a.C, a.D, a.N, BWD, p);
+    gn_plan_resident(a.HW, a.C, a.D, a.N, BWD ? kGnBwdRegs<TANH> : kGnFwdRegs, p);
     if (p.resident && !(gn_aligned(a.x) && gn_aligned(a.out) && gn_aligned(a.gamma) && gn_aligned(a.beta) && (!BWD || gn_aligned(a.dy))))
         p.resident = false;
     long part_rows;
@@ -576,6 +580,8 @@ extern "C" int mmdgan_gn_fwd(const float *x, int N, long HW, int C, int G, const
     MMDGAN_REQUIRE(x && gamma && beta && y && stats && workspace, "gn_fwd: null pointer");
     GN_REQUIRE_GEOMETRY("gn_fwd");
     MMDGAN_REQUIRE(eps > 0.f, "gn_fwd: eps must be positive");
+    const size_t bytes = (size_t)N * HW * C * 4;
+    MMDGAN_REQUIRE(y == x || !spans_meet(y, bytes, x, bytes), "gn_fwd: y overlaps x without being x");
     GnArgs a{};
     a.x = x; a.gamma = gamma; a.beta = beta; a.stats = stats; a.out = y;
     a.N = a.x_batch = N; a.HW = (int)HW; a.C = C; a.G = G; a.D = C / G; a.eps = eps;
@@ -589,6 +595,10 @@ extern "C" int mmdgan_gn_bwd(const float *x, const float *dy, int N, int x_batch
     if (x_batch == 0) x_batch = N;
     MMDGAN_REQUIRE(x_batch >= 1 && x_batch <= N && N - x_batch <= x_batch, "gn_bwd: x_batch %d for %d images", x_batch, N);
     MMDGAN_REQUIRE(dx != x || x_batch == N, "gn_bwd: dx must not be x when images of x are read twice");
+    const size_t bytes = (size_t)N * HW * C * 4;
+    MMDGAN_REQUIRE((dx == x || !spans_meet(dx, bytes, x, (size_t)x_batch * HW * C * 4)) && (dx == dy || !spans_meet(dx, bytes, dy, bytes)),
+                   "gn_bwd: dx overlaps x or dy without being it");
+    MMDGAN_REQUIRE(!dgamma || !dbeta || !spans_meet(dgamma, (size_t)C * 4, dbeta, (size_t)C * 4), "gn_bwd: dgamma overlaps dbeta");
     GnArgs a{};
     a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.stats = const_cast<double *>(stats); a.out = dx;
     a.N = N; a.x_batch = x_batch; a.HW = (int)HW; a.C = C; a.G = G; a.D = C / G;

@@ -552,12 +552,16 @@ static MuMat mu_place(int rows, int cols, bool keep_u, int steps, size_t base) {
     const long n = (long)rows * cols, want = (n + kMuPrepPer - 1) / kMuPrepPer;
     m.nparts = (int)(want < kMuPrepMax ? want : kMuPrepMax);
     // one triangle of 128 x 128 tiles, the reduction in runs of 8 to 16 32-wide steps: 512 workgroups from one matrix where it has
-    // them, and no run so short that its 64 KB of sums cost more than its 32 KB stages.  (A rule on the matrix alone: what it
-    // gives does not depend on the others of a call.)
+    // them, and no run so short that its 64 KB of sums cost more than its 32 KB stages; up to 64 steps where 4096 workgroups
+    // remain (4194304 x 511: 34.9 ms and 37 GB of scratch, with 16 steps 38.5 ms and 41 GB).  (A rule on the matrix alone:
+    // what it gives does not depend on the others of a call.)
     const int tb = m.mp / 128, all = m.np / 32;
     m.tiles = tb * (tb + 1) / 2;
     long run = ((long)m.tiles * all + 511) / 512;
-    run = run < 8 ? 8 : run > 16 ? 16 : (run + 1) & ~1L;     // (even: mu_tile)
+    run = run < 8 ? 8 : run > 16 ? 16 : run;
+    const long far = (long)m.tiles * all / 4096;
+    if (far > run) run = far < 64 ? far : 64;
+    run = (run + 1) & ~1L;                                   // (even: mu_tile)
     m.steps_per = all < run ? all : (int)run;
     m.splits = (all + m.steps_per - 1) / m.steps_per;
     const size_t bx = m.mp / 32 * mu_strip(m.np / 16) * 2, bt = m.np / 32 * mu_strip(m.mp / 16) * 2, sq = m.mp / 32 * mu_strip(m.mp / 16) * 2;
@@ -771,6 +775,26 @@ static int mu_check(const mmdgan_muon_job *jobs, int n_jobs, int steps, bool upd
         MMDGAN_REQUIRE(j.grad && j.out, "%s: matrix %d: null pointer", what, i);
         MMDGAN_REQUIRE(!update || (j.param && j.momentum && j.momentum_out), "%s: matrix %d: null pointer", what, i);
         MMDGAN_REQUIRE(!j.dsigma || (j.dot && j.sigma && j.scale), "%s: matrix %d: dsigma without dot, sigma and scale", what, i);
+    }
+    // what a matrix writes is its own: groups run one after the other, and a matrix's workgroups in no order
+    for (int i = 0; i < n_jobs; ++i) {
+        const mmdgan_muon_job &j = jobs[i];
+        const size_t bytes = (size_t)j.rows * j.cols * 4;
+        for (int k = 0; k < n_jobs; ++k) {
+            const mmdgan_muon_job &o = jobs[k];
+            const size_t ob = (size_t)o.rows * o.cols * 4;
+            const bool same = i == k;
+            bool meet = (same ? (update || j.out != o.grad) && spans_meet(j.out, bytes, o.grad, ob)
+                              : spans_meet(j.out, bytes, o.grad, ob) || spans_meet(j.out, bytes, o.out, ob));
+            if (update) {
+                meet = meet || (!(same && j.out == o.param) && spans_meet(j.out, bytes, o.param, ob)) || spans_meet(j.out, bytes, o.momentum, ob) ||
+                       spans_meet(j.out, bytes, o.momentum_out, ob) || spans_meet(j.out, bytes, o.dsigma, ob);
+                meet = meet || spans_meet(j.momentum_out, bytes, o.grad, ob) || spans_meet(j.momentum_out, bytes, o.param, ob) ||
+                       (!(same && j.momentum_out == o.momentum) && spans_meet(j.momentum_out, bytes, o.momentum, ob)) ||
+                       (!same && spans_meet(j.momentum_out, bytes, o.momentum_out, ob)) || spans_meet(j.momentum_out, bytes, o.dsigma, ob);
+            }
+            MMDGAN_REQUIRE(!meet, "%s: an output of matrix %d overlaps a tensor of matrix %d", what, i, k);
+        }
     }
     return MMDGAN_OK;
 }

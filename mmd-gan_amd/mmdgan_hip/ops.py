@@ -483,9 +483,17 @@ def group_norm_workspace(N, HW, C, groups, device):
     return torch.empty(n, device=device, dtype=torch.uint8)
 
 
+def _on_current_device(*tensors):
+    """launches go to the current device's current stream: a tensor that lives on another one is refused"""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        assert t is None or t.get_device() == here, 'a tensor lives on device {}, the current one is {}'.format(t.get_device(), here)
+
+
 def _gn_geometry(x, gamma, beta, groups):
     assert x.dim() >= 2, 'group_norm: x is [N, ..., C], channels last'
     N, C = x.shape[0], x.shape[-1]
+    assert max(N, C) < 1 << 31, 'group_norm: {} images of {} channels'.format(N, C)      # (they travel as C ints)
     assert gamma.numel() == C and beta.numel() == C, 'group_norm: gamma and beta have one entry per channel'
     HW = 1
     for s in x.shape[1:-1]:
@@ -517,8 +525,10 @@ def group_norm_fwd(x, gamma, beta, groups, act='linear', eps=1e-5, out=None, sta
     y = out if out is not None else torch.empty_like(x)
     assert y.shape == x.shape
     st = stats if stats is not None else torch.empty((N, max(G, 0), 2), device=x.device, dtype=torch.float64)
+    ws = _gn_ws(workspace, N, HW, C, G, x.device)
+    _on_current_device(x, gamma, beta, y, st, ws)
     check(lib.mmdgan_gn_fwd(_p(x), N, HW, C, G, _p(gamma), _p(beta), float(eps), act_id(act), _p(y), _p64(st, (N, G, 2)),
-                            _gn_ws(workspace, N, HW, C, G, x.device).data_ptr(), _stream()), 'group_norm_fwd')
+                            ws.data_ptr(), _stream()), 'group_norm_fwd')
     return y, st
 
 
@@ -538,8 +548,10 @@ def group_norm_bwd(x, dy, gamma, beta, stats, act='linear', out=None, dgamma=Non
         assert dgamma.numel() == C and dbeta.numel() == C
     else:
         dgamma = dbeta = None
+    ws = _gn_ws(workspace, N, HW, C, G, x.device)
+    _on_current_device(x, dy, gamma, beta, stats, dx, dgamma, dbeta, ws)
     check(lib.mmdgan_gn_bwd(_p(x), _p(dy), N, xb, HW, C, G, _p(gamma), _p(beta), _p64(stats, (xb, G, 2)), act_id(act), _p(dx),
-                            _p(dgamma), _p(dbeta), _gn_ws(workspace, N, HW, C, G, x.device).data_ptr(), _stream()), 'group_norm_bwd')
+                            _p(dgamma), _p(dbeta), ws.data_ptr(), _stream()), 'group_norm_bwd')
     return dx, dgamma, dbeta
 
 
@@ -859,7 +871,10 @@ def _matrix_shape(t):
 def _muon_jobs(tensors):
     jobs = (MuonJob * len(tensors))()
     for j, t in zip(jobs, tensors):
-        j.rows, j.cols = _matrix_shape(t)
+        rows, cols = _matrix_shape(t)
+        if max(rows, cols) >= 1 << 31:                       # (they travel as C ints)
+            raise ValueError('orthogonalised updates: a matrix of %dx%d' % (rows, cols))
+        j.rows, j.cols = rows, cols
     return jobs
 
 
@@ -884,7 +899,7 @@ def orthogonalize_workspace(mats, steps=5):
 def orthogonalize(mats, steps=5, out=None, workspace=None):
     """O for every matrix of a list (or for one tensor): singular values taken to about 1 by `steps` iterates of a quintic, singular
     vectors kept (mmdgan_orthogonalize).  A tensor of more than two dimensions is its [prod(shape[:-1]), shape[-1]] view.
-    Returns tensors of the same shapes; out may be the inputs."""
+    Returns tensors of the same shapes; out may be the inputs, each its own."""
     lib = require_device()
     single = torch.is_tensor(mats)
     mats = [mats] if single else list(mats)
@@ -896,6 +911,7 @@ def orthogonalize(mats, steps=5, out=None, workspace=None):
     for j, t, o in zip(jobs, mats, outs):
         j.grad, j.out = _p(t), _p(o)
     ws = _muon_ws(jobs, steps, mats[0].device, workspace)
+    _on_current_device(ws, *mats, *outs)
     check(lib.mmdgan_orthogonalize(ctypes.cast(jobs, ctypes.c_void_p), len(jobs), int(steps), ws.data_ptr(), _stream()),
           'orthogonalize')
     return outs[0] if single else outs
@@ -919,9 +935,10 @@ class MuonGroup:
         self._jobs = _muon_jobs(params)
         for j, p, g, m, f, po, mo in zip(self._jobs, *self.keep):
             assert p.shape == g.shape == m.shape == po.shape == mo.shape
+            assert len({t.get_device() for t in (params[0], p, g, m, po, mo)}) == 1, 'tensors on several devices'
             j.param, j.grad, j.momentum, j.out, j.momentum_out = _p(p), _p(g), _p(m), _p(po), _p(mo)
             if f is not None:
-                assert f['dsigma'].numel() == p.numel()
+                assert f['dsigma'].numel() == p.numel() and len({t.get_device() for t in (p, f['dsigma'], f['dot'], f['sigma'], f['scale'])}) == 1
                 j.dsigma, j.dot, j.sigma, j.scale = (_p(f[k]) for k in ('dsigma', 'dot', 'sigma', 'scale'))
         self._ws = {}
 
@@ -935,6 +952,7 @@ class MuonGroup:
                 workspace = self._ws[steps] = _muon_ws(self._jobs, steps, self.keep[0][0].device)
         else:
             _muon_ws(self._jobs, steps, None, workspace)
+        _on_current_device(self.keep[0][0], workspace)
         check(lib.mmdgan_muon_update(ctypes.cast(self._jobs, ctypes.c_void_p), len(self._jobs), float(lr), float(momentum), int(bool(nesterov)),
                                      float(weight_decay), float(grad_scale), int(self.fold_fixup), int(steps),
                                      workspace.data_ptr(), _stream()), 'muon_update')

@@ -69,14 +69,25 @@ def batch(arch, B, rs):
 
 @pytest.mark.parametrize('make,mode', [(dcgan_gn, 'eager'), (lambda: dcgan_gn(8), 'plan'), (resnet_gn, 'eager'), (resnet_gn, 'plan')])
 def test_step_with_group_norm_matches_the_oracle(make, mode):
-    """three steps, each from the oracle's variables: images, losses and every gradient at the bars of the other engine tests
+    """three steps, each from the oracle's variables: images, scores, losses and every gradient at the bars of the other engine tests
     (1e-4 of a tensor in L2; the losses' floor of 4e-7 of their kernel means).  lrelu and tanh: no activation whose derivative
-    a rounding could switch off entirely"""
+    a rounding could switch off entirely.
+    What a loss may be off by has two parts.  |L - ref| <= |L - L64(s)| + |L64(s) - L64(s_ref)| with s the engine's scores, L64 the loss in
+    64 bits: the first is the loss kernel's, held to the bar above; the second is what scores that are right to fp32 make of a loss
+    that amplifies them.  The kernels here are exp(-d^2 / 2) with means of 5e-4, so d^2 / 2 is about 8 and a relative error e of the
+    distances is one of 16 e in every mean; the loss is a difference of means 15 times as large: 240 e, 1e-4 already at e = 4e-7 = 7 *
+    2^-24, less than ten layers of sums of up to 512 fp32 terms leave (sqrt(512) roundings each, 1.4e-6; ten in quadrature 4e-6).  So s itself is held in L2, and L64(s) to 240 * 4e-6 = 1e-3."""
     arch, B = make(), 8
     eng = engine(arch, B, launch_mode=mode)
     ora = R.OracleGan(arch, 'rep', (5e-4, 2e-4), dtype=torch.float64, params=eng.get_variables())
     assert sorted(ora.params) == sorted(eng.variable_names())
     assert any('/GN/gamma' in n for n in eng.variable_names()) and eng._d_joint      # (rows of D stay independent under group norm)
+    launch, seen = eng._loss.launch, []
+
+    def keep_scores(scores, *a, **kw):                       # (a plan calls it once: its replays write the same buffer)
+        seen[:] = [scores, scores.clone()]
+        return launch(scores, *a, **kw)
+    eng._loss.launch = keep_scores
     rs = np.random.RandomState(5)
     for step in range(3):
         z, real = batch(arch, B, rs)
@@ -88,8 +99,14 @@ def test_step_with_group_norm_matches_the_oracle(make, mode):
         fake = np.transpose(eng._dis_in[B:].cpu().numpy(), (0, 3, 1, 2))
         assert np.abs(fake - gen.detach().numpy()).max() <= 1e-4 * np.abs(gen.detach().numpy()).max()
         got = eng.losses.cpu().numpy().astype(np.float64)
-        for i, ref in enumerate((float(lg), float(ld))):
-            assert abs(got[i] - ref) <= 1e-4 * abs(ref) + 4e-7 * float(max(got[2:5])), (step, i, got[i], ref)
+        assert mode == 'plan' and step or torch.equal(*seen)                             # (the scores outlive the step)
+        s, s64 = seen[0].cpu().double(), torch.cat([s_x, s_gen]).detach()
+        assert (s - s64).norm() <= 1e-4 * s64.norm(), step
+        own = R.gan_loss(s[B:], s[:B], 'rep', B, rep_weights=eng.rep_weights)
+        for i, (ref, mine) in enumerate(zip((float(lg), float(ld)), own)):
+            bar = 4e-7 * float(max(got[2:5]))
+            assert abs(got[i] - float(mine)) <= 1e-4 * abs(float(mine)) + bar, (step, i, got[i], float(mine))
+            assert abs(float(mine) - ref) <= 1e-3 * abs(ref) + bar, (step, i, float(mine), ref)
         if step == 0:
             continue                                     # (gradients of un-normalised start vectors: rounding noise, as in the other step tests)
         grads = eng.get_variables(grad=True)

@@ -67,3 +67,84 @@ def test_orthogonalised_updates_refuse_bad_jobs(lib):
     assert lib.mmdgan_orthogonalize(None, 1, 5, 16, None) == -1
     size = lambda steps=5, **kw: lib.mmdgan_muon_workspace_bytes(job(**kw)[0], 1, steps)
     assert size() > 0 and size(steps=0) == 0 and size(rows=0) == 0 and size(rows=9000, cols=9000) == 0
+
+
+def test_group_norm_refuses_overlaps(lib):
+    A, B, size = 1 << 20, 1 << 22, 4 * 9 * 12 * 4           # addresses that are only compared
+
+    def fwd(y):
+        return lib.mmdgan_gn_fwd(A, 4, 9, 12, 3, 16, 16, 1e-5, 0, y, 16, 16, None)
+
+    def bwd(dx, xb=4, dgamma=None, dbeta=None):
+        return lib.mmdgan_gn_bwd(A, B, 4, xb, 9, 12, 3, 16, 16, 16, 0, dx, dgamma, dbeta, 16, None)
+    for call in (lambda: fwd(A + 16), lambda: fwd(A - size + 4), lambda: fwd(A + size - 4), lambda: bwd(A + 16), lambda: bwd(A - size + 4),
+                 lambda: bwd(B + 16), lambda: bwd(B + size - 4), lambda: bwd(1 << 24, 4, 1 << 25, (1 << 25) + 44)):
+        assert call() == -1 and 'overlap' in message(lib)
+    assert bwd(A, xb=2) == -1 and 'dx must not be x' in message(lib)
+
+
+def test_orthogonalised_updates_refuse_overlaps(lib):
+    """an output may be its own matrix's input, and overlaps nothing else: another matrix reads it at a time that is not fixed"""
+    import ctypes
+    from mmdgan_hip.ops import MuonJob
+    base, size = 1 << 20, 8 * 100 * 4                        # addresses that are only compared
+    names = ('grad', 'out', 'param', 'momentum', 'momentum_out', 'dsigma')
+
+    def jobs(*change):
+        j = (MuonJob * 2)()
+        for i in range(2):
+            for k, f in enumerate(names):
+                setattr(j[i], f, base + (i * 8 + k) * 4096)
+            j[i].dot = j[i].sigma = j[i].scale = base - 64
+            j[i].rows, j[i].cols = (8, 100) if i == 0 else (100, 8)
+        for i, f, i2, f2, off in change:
+            setattr(j[i], f, getattr(j[i2], f2) + off)
+        return ctypes.cast(j, ctypes.c_void_p), j
+
+    def orth(*change):
+        p, keep = jobs(*change)
+        return lib.mmdgan_orthogonalize(p, 2, 5, 16, None)
+
+    def update(*change):
+        p, keep = jobs(*change)
+        return lib.mmdgan_muon_update(p, 2, 0.1, 0.9, 1, 0.0, 1.0, 1, 5, 16, None)
+    for change in ((0, 'out', 1, 'grad', 0), (1, 'out', 0, 'grad', 0), (0, 'out', 1, 'out', 0), (0, 'out', 0, 'grad', 16),
+                   (1, 'out', 1, 'grad', 4 - size), (1, 'out', 0, 'grad', size - 4)):
+        assert orth(change) == -1 and 'overlaps' in message(lib), change
+    for a in ('out', 'momentum_out'):
+        for i in range(2):
+            for k in range(2):
+                for b in names:
+                    own = i == k and (a, b) in (('out', 'param'), ('momentum_out', 'momentum'))
+                    for off in (16, 4 - size) if own else () if i == k and a == b else (0, 16, size - 4):
+                        assert update((i, a, k, b, off)) == -1 and 'overlaps' in message(lib), (i, a, k, b, off)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    """launches go to the current device: the check itself, with stand-ins for tensors"""
+    import torch
+    from mmdgan_hip import ops
+
+    class T:
+        def __init__(self, d):
+            self.d = d
+
+        def get_device(self):
+            return self.d
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 1)
+    ops._on_current_device(T(1), None, T(1))
+    for bad in ((T(0),), (T(1), T(0)), (T(1), None, T(-1))):
+        with pytest.raises(AssertionError, match='device'):
+            ops._on_current_device(*bad)
+
+
+def test_sides_that_do_not_fit_an_int_are_refused():
+    import torch
+    from mmdgan_hip import ops
+    wide = torch.empty(1, device='meta').expand(1 << 33, 2)
+    for t in (wide, wide.t()):
+        with pytest.raises(ValueError, match='8589934592'):
+            ops._muon_jobs([t])
+    g = torch.empty(1, device='meta').expand((1 << 32) + 4)
+    with pytest.raises(AssertionError, match='4294967300'):
+        ops._gn_geometry(g[None], g, g, 4)
