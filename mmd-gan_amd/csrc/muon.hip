@@ -32,6 +32,10 @@ typedef unsigned int mu_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMuPad = 128;
 constexpr int kMuChain = 3;                  // steps between two true Gram matrices
+// X <- P X in tiles of 128 x 128; of 64 x 128 where a launch has fewer than 512 of the former (two on a CU at once): 129x1001
+// alone 131 -> 119 us, 4608x512 171 -> 163.  On a net's matrices together the finer tiles change nothing or cost: they read half
+// as much again per product (64x64 images' discriminator 0.99 -> 1.00 ms).
+constexpr int kMuApplyFine = 512;
 constexpr float kScaleX = 4096.f, kScaleA = 4096.f, kScaleQ = 8192.f, kScaleP = 1024.f;
 
 // halves from one row block to the next, of `kb` = K / 16 blocks
@@ -55,54 +59,57 @@ __device__ __forceinline__ void mu_put8(f16 *o, size_t at, const float (&v)[8]) 
 }
 
 // ---- the product of one tile -------------------------------------------------------------------------------------
-// C[i, j] = sum_k A[i, k] B[j, k] for a 128 x 128 tile, four waves as 2 x 2 of 64 x 64.  Per 32-wide step the workgroup stages four row
-// blocks of each operand (4 KB each, contiguous in memory) in LDS, double buffered.  a / b: the first block of the tile's first row
-// block; sa / sb: halves from one row block to the next.
-constexpr int kMuStage = 8 * 4096;                           // bytes of a stage: four row blocks of a, four of b
-__device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, size_t sb, int steps, char *lds, f32x16 (&acc)[2][2]) {
+// C[i, j] = sum_k A[i, k] B[j, k] for a tile of 64 TA x 128, four waves as 2 x 2 of 32 TA x 64.  Per 32-wide step the workgroup stages
+// 2 TA row blocks of a and four of b (4 KB each, contiguous in memory) in LDS, double buffered.  a / b: the first block of the tile's
+// first row block; sa / sb: halves from one row block to the next.
+template <int TA> constexpr int kMuStage = (2 * TA + 4) * 4096;      // bytes of a stage
+template <int TA>
+__device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, size_t sb, int steps, char *lds, f32x16 (&acc)[TA][2]) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    mu_u32x4 ga[4], gb[4];
+    mu_u32x4 ga[2 * TA], gb[4];
     auto fetch = [&](int s) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            ga[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
+            if (i < 2 * TA) ga[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
             gb[i] = *reinterpret_cast<const mu_u32x4 *>(b + i * sb + (size_t)s * 2048 + t * 8);
         }
     };
     auto store = [&](char *buf) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<mu_u32x4 *>(buf + i * 4096 + t * 16) = ga[i];
-            *reinterpret_cast<mu_u32x4 *>(buf + (4 + i) * 4096 + t * 16) = gb[i];
+            if (i < 2 * TA) *reinterpret_cast<mu_u32x4 *>(buf + i * 4096 + t * 16) = ga[i];
+            *reinterpret_cast<mu_u32x4 *>(buf + (2 * TA + i) * 4096 + t * 16) = gb[i];
         }
     };
-    f32x16 low[2][2];                                        // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
+    f32x16 low[TA][2];                                       // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TA; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) { acc[i][j] = f32x16{}; low[i][j] = f32x16{}; }
-    const int ar = (w >> 1) * 2 * 4096 + lane * 16, br = (4 + (w & 1) * 2) * 4096 + lane * 16;
-    struct Frag { f16x8 ah[2], al[2], bh[2], bl[2]; } f0, f1;
+    const int ar = (w >> 1) * TA * 4096 + lane * 16, br = (2 * TA + (w & 1) * 2) * 4096 + lane * 16;
+    struct Frag { f16x8 ah[TA], al[TA], bh[2], bl[2]; } f0, f1;
     auto read = [&](Frag &f, const char *buf, int ks) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            f.ah[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048);
-            f.al[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048 + 1024);
+            if (i < TA) {
+                f.ah[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048);
+                f.al[i] = *reinterpret_cast<const f16x8 *>(buf + ar + i * 4096 + ks * 2048 + 1024);
+            }
             f.bh[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048);
             f.bl[i] = *reinterpret_cast<const f16x8 *>(buf + br + i * 4096 + ks * 2048 + 1024);
         }
     };
-    auto multiply = [&](const Frag &f) {                     // (an accumulator is touched every fourth product)
+    auto multiply = [&](const Frag &f) {                     // (an accumulator is touched every 2 TA-th product)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], low[i][j], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], low[i][j], 0, 0, 0);
     };
@@ -115,7 +122,7 @@ __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, s
     lds_barrier();
     read(f0, lds, 0);
     for (int s = 0; s < steps; ++s) {
-        char *cur = lds + (s & 1) * kMuStage, *nxt = lds + ((s + 1) & 1) * kMuStage;
+        char *cur = lds + (s & 1) * kMuStage<TA>, *nxt = lds + ((s + 1) & 1) * kMuStage<TA>;
         const bool more = s + 1 < steps;
         read(f1, cur, 1);
         multiply(f0);
@@ -127,7 +134,7 @@ __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, s
     }
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TA; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] += low[i][j];
 }
@@ -186,9 +193,10 @@ __device__ __forceinline__ double mu_prep_one(const MuPrep &p, const MuPrepTable
 // grad_scale * (scale * grad - (scale / sigma) <grad, W> dsigma/dW)  (Adam's read, elementwise.hip).  HBM-bound.
 __global__ __launch_bounds__(256) void mu_prep_kernel(MuPrepTable t) {
     __shared__ double red[4];
-    const int q = mu_which(t.f, blockIdx.x);
-    const MuPrep &p = t.j[q];
-    const unsigned nb = p.blocks, b = blockIdx.x - t.f.first[q];
+    MuPrep p;
+    unsigned start;
+    mu_which(t.f, t.j, blockIdx.x, p, start);
+    const unsigned nb = p.blocks, b = blockIdx.x - start;
     float c0 = t.grad_scale, c1 = 0.f;
     if (p.dsigma) { c0 = t.grad_scale * p.scale[0]; c1 = t.grad_scale * (p.scale[0] / p.sigma[0]) * p.dot[0]; }
     double ss = 0.0;
@@ -251,33 +259,39 @@ struct MuSplitTable { MuFirst<kMuGroup> f; MuSplit j[kMuGroup]; };
 __global__ __launch_bounds__(256) void mu_split_kernel(MuSplitTable t) {
     __shared__ float tile[64][65];
     __shared__ double s_sum[4];
-    const int q = mu_which(t.f, blockIdx.x);
-    const MuSplit &p = t.j[q];
-    const int b = blockIdx.x - t.f.first[q];
+    MuSplit p;
+    unsigned start;
+    mu_which(t.f, t.j, blockIdx.x, p, start);
+    const int b = blockIdx.x - start;
     const int prows = p.tall ? p.np : p.mp, pcols = p.tall ? p.mp : p.np;
     const int r0 = b / (pcols / 64) * 64, c0 = b % (pcols / 64) * 64;
-    double ss = 0.0;
+    // everything asked for before anything is waited for: the partial sums, this thread's sixteen values (clamped, not skipped)
+    const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6, c = c0 + tc < p.cols ? c0 + tc : p.cols - 1;
+    double d[kMuPrepMax / 256];
+    float u[16];
 #pragma unroll
     for (int i = 0; i < kMuPrepMax / 256; ++i) {
         const int at = threadIdx.x + 256 * i;
-        ss += at < p.nparts ? p.part[at] : 0.0;
+        d[i] = p.part[at < p.nparts ? at : 0];
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = r0 + tr + 4 * i;
+        u[i] = p.u[(size_t)(r < p.rows ? r : p.rows - 1) * p.cols + c];
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < kMuPrepMax / 256; ++i) ss += (int)threadIdx.x + 256 * i < p.nparts ? d[i] : 0.0;
     ss = wave_sum(ss);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = ss;
     f16 *nat = p.tall ? p.xt : p.x, *tra = p.tall ? p.x : p.xt;
+    __syncthreads();
     {
-        const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6;
-        float u[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = r0 + tr + 4 * i, c = c0 + tc;
-            u[i] = r < p.rows && c < p.cols ? p.u[(size_t)r * p.cols + c] : 0.f;
-        }
-        __syncthreads();
         const double s = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
         const double inv = s > 0.0 ? (double)kScaleX / sqrt(s) : s == 0.0 ? 0.0 : s;                 // (NaN stays NaN)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) tile[tr + 4 * i][tc] = (float)((double)u[i] * inv);
+        for (int i = 0; i < 16; ++i)
+            tile[tr + 4 * i][tc] = r0 + tr + 4 * i < p.rows && c0 + tc < p.cols ? (float)((double)u[i] * inv) : 0.f;
     }
     __syncthreads();
     // a lane writes 8 values along the operand's own k: lane = row % 32 + 32 * (k / 8 % 2), as the blocks are laid out
@@ -305,10 +319,11 @@ struct MuGram {
 struct MuGramTable { MuFirst<kMuGroup> f, r; MuGram j[kMuGroup]; };
 
 __global__ __launch_bounds__(256, 2) void mu_gram_kernel(MuGramTable t) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage];
-    const int q = mu_which(t.f, blockIdx.x);
-    const MuGram &p = t.j[q];
-    const int b = mu_item(blockIdx.x - t.f.first[q], p.tiles * p.splits);
+    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage<2>];
+    MuGram p;
+    unsigned start;
+    mu_which(t.f, t.j, blockIdx.x, p, start);
+    const int b = mu_item(blockIdx.x - start, p.tiles * p.splits);
     if (b < 0) return;
     const int split = b / p.tiles, tile = b % p.tiles;
     int ti, tj;
@@ -317,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void mu_gram_kernel(MuGramTable t) {
     const int steps = s0 + p.steps_per < all ? p.steps_per : all - s0;
     f32x16 acc[2][2];
     const size_t sx = mu_strip(p.np / 16);
-    mu_tile(p.x + (size_t)ti * 4 * sx + (size_t)s0 * 2048, sx, p.x + (size_t)tj * 4 * sx + (size_t)s0 * 2048, sx, steps, lds, acc);
+    mu_tile<2>(p.x + (size_t)ti * 4 * sx + (size_t)s0 * 2048, sx, p.x + (size_t)tj * 4 * sx + (size_t)s0 * 2048, sx, steps, lds, acc);
     float *o = p.slab + ((size_t)split * p.tiles + tile) * 128 * 128;
     const int w = threadIdx.x >> 6;
 #pragma unroll
@@ -332,9 +347,10 @@ __global__ __launch_bounds__(256, 2) void mu_gram_kernel(MuGramTable t) {
 // sums the splits of a 32 x 32 block in order, writes A packed, and its mirror image
 __global__ __launch_bounds__(256) void mu_gram_reduce_kernel(MuGramTable t) {
     __shared__ float blk[32][33];
-    const int q = mu_which(t.r, blockIdx.x);
-    const MuGram &p = t.j[q];
-    const int b = blockIdx.x - t.r.first[q], tile = b >> 4, sub = b & 15;
+    MuGram p;
+    unsigned start;
+    mu_which(t.r, t.j, blockIdx.x, p, start);
+    const int b = blockIdx.x - start, tile = b >> 4, sub = b & 15;
     int ti, tj;
     mu_tri(tile, ti, tj);
     const int r0 = (sub >> 2) * 32, c0 = (sub & 3) * 32, tc = (threadIdx.x & 7) * 4, tr = threadIdx.x >> 3;
@@ -401,9 +417,10 @@ __device__ __forceinline__ int mu_lds32(int r, int c) { return r * 32 + (((c >> 
 
 __global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
     __shared__ __attribute__((aligned(16))) float part[4][32 * 32];
-    const int q = mu_which(t.f, blockIdx.x);
-    const MuSquare &p = t.j[q];
-    const int item = mu_item(blockIdx.x - t.f.first[q], p.tiles);
+    MuSquare p;
+    unsigned start;
+    mu_which(t.f, t.j, blockIdx.x, p, start);
+    const int item = mu_item(blockIdx.x - start, p.tiles);
     if (item < 0) return;
     int ti, tj;
     mu_tri_blocked(item, p.mp / 32, ti, tj);
@@ -475,25 +492,26 @@ struct MuApply {
 };
 struct MuApplyTable { MuFirst<kMuGroup> f; MuApply j[kMuGroup]; };
 
-template <bool LAST>
+template <bool LAST, int TA>
 __global__ __launch_bounds__(256, 2) void mu_apply_kernel(MuApplyTable t) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage];
-    const int q = mu_which(t.f, blockIdx.x);
-    const MuApply &p = t.j[q];
-    const int b = mu_item(blockIdx.x - t.f.first[q], p.items), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ __attribute__((aligned(16))) char lds[2 * kMuStage<TA>];
+    MuApply p;
+    unsigned start;
+    mu_which(t.f, t.j, blockIdx.x, p, start);
+    const int b = mu_item(blockIdx.x - start, p.items), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     if (b < 0) return;
     // the m side of the tile runs fastest: its operand (P, at most a few MB) stays in L2 while X streams through once
-    const int tr = (LAST && p.flip ? b / p.tiles_m : b % p.tiles_m) * 128, tc = (LAST && p.flip ? b % p.tiles_m : b / p.tiles_m) * 128;
+    const int tr = (LAST && p.flip ? b / p.tiles_m : b % p.tiles_m) * 64 * TA, tc = (LAST && p.flip ? b % p.tiles_m : b / p.tiles_m) * 128;
     const size_t sr = mu_strip(p.mp / 16);
-    f32x16 acc[2][2];
-    mu_tile(p.a + (size_t)(tr / 32) * sr, sr, p.b + (size_t)(tc / 32) * sr, sr, p.mp / 32, lds, acc);
-    const int r0 = tr + (w >> 1) * 64, c0 = tc + (w & 1) * 64;           // this wave's 64 x 64
+    f32x16 acc[TA][2];
+    mu_tile<TA>(p.a + (size_t)(tr / 32) * sr, sr, p.b + (size_t)(tc / 32) * sr, sr, p.mp / 32, lds, acc);
+    const int r0 = tr + (w >> 1) * 32 * TA, c0 = tc + (w & 1) * 64;      // this wave's 32 TA x 64
     if (LAST) {
         // (every parameter is read before the first result is written: out may be param)
-        float old[2][2][16];
+        float old[TA][2][16];
         if (p.param) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -503,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void mu_apply_kernel(MuApplyTable t) {
                     }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -515,21 +533,24 @@ __global__ __launch_bounds__(256, 2) void mu_apply_kernel(MuApplyTable t) {
         return;
     }
     // both layouts of the next X from the wave's own quarter of the staging buffers (mu_tile ends with a barrier)
-    float *mine = reinterpret_cast<float *>(lds) + w * 4096;
+    float *mine = reinterpret_cast<float *>(lds) + w * 2048 * TA;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TA; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mine[mu_lds(i * 32 + mu_row(e), j * 32 + mu_col())] = p.alpha * acc[i][j][e];
     __syncthreads();
 #pragma unroll
-    for (int blk = 0; blk < 8; ++blk) {
-        const int r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
+    for (int blk = 0; blk < 4 * TA; ++blk) {
         float v[8];
+        {
+            const int r = (blk >> 2) * 32 + (lane & 31), k = (blk & 3) * 16 + (lane >> 5) * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = mine[mu_lds(r, k) + e];
-        mu_put8(p.x, mu_off(r0 + r, c0 + k, p.np / 16), v);
+            for (int e = 0; e < 8; ++e) v[e] = mine[mu_lds(r, k) + e];
+            mu_put8(p.x, mu_off(r0 + r, c0 + k, p.np / 16), v);
+        }
+        const int r = (blk / (2 * TA)) * 32 + (lane & 31), k = (blk % (2 * TA)) * 16 + (lane >> 5) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = mine[mu_lds(k + e, r)];
         mu_put8(p.xt, mu_off(c0 + r, r0 + k, p.mp / 16), v);
@@ -638,7 +659,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
         const int chain = steps - done < kMuChain ? steps - done : kMuChain;
         {
             MuGramTable t{};
-                unsigned blocks = 0, red = 0;
+            unsigned blocks = 0, red = 0;
             for (int i = 0; i < n; ++i) {
                 MuGram &p = t.j[i];
                 p.x = x[i]; p.slab = (float *)(ws + m[i].slab); p.a = (f16 *)(ws + m[i].a);
@@ -696,6 +717,9 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
         done += chain;
         MuApplyTable t{};
         unsigned blocks = 0;
+        long all = 0;
+        for (int i = 0; i < n; ++i) all += (long)(m[i].mp / 128) * (m[i].np / 128);
+        const int ta = all < kMuApplyFine ? 1 : 2;
         const float s_p = chain == 1 ? kScaleQ : kScaleP;
         for (int i = 0; i < n; ++i) {
             MuApply &p = t.j[i];
@@ -703,17 +727,23 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
             const bool flip = done == steps && m[i].tall;    // the result in U's own layout: tile rows along its rows
             p.a = flip ? xt[i] : pp; p.b = flip ? pp : xt[i];
             p.mp = m[i].mp; p.np = m[i].np; p.rows = jobs[i].rows; p.cols = jobs[i].cols;
-            p.tiles_m = m[i].mp / 128; p.flip = flip;
+            p.flip = flip;
+            p.tiles_m = flip ? m[i].mp / 128 : m[i].mp / (64 * ta);
             p.alpha = done == steps ? 1.f / (s_p * kScaleX) : 1.f / s_p;
             p.x = x[i]; p.xt = xt_next[i];
             p.param = update ? jobs[i].param : nullptr; p.out = jobs[i].out; p.keep = jobs[i].keep; p.step = jobs[i].step;
             t.f.first[i] = blocks;
-            p.items = m[i].mp / 128 * (m[i].np / 128);
+            p.items = m[i].mp / 128 * (m[i].np / 128) * (2 / ta);
             blocks += (unsigned)(p.items + 7) & ~7u;
         }
         mu_close(t.f, n);
-        if (done == steps) hipLaunchKernelGGL((mu_apply_kernel<true>), dim3(blocks), dim3(256), 0, st, t);
-        else hipLaunchKernelGGL((mu_apply_kernel<false>), dim3(blocks), dim3(256), 0, st, t);
+        if (ta == 1) {
+            if (done == steps) hipLaunchKernelGGL((mu_apply_kernel<true, 1>), dim3(blocks), dim3(256), 0, st, t);
+            else hipLaunchKernelGGL((mu_apply_kernel<false, 1>), dim3(blocks), dim3(256), 0, st, t);
+        } else {
+            if (done == steps) hipLaunchKernelGGL((mu_apply_kernel<true, 2>), dim3(blocks), dim3(256), 0, st, t);
+            else hipLaunchKernelGGL((mu_apply_kernel<false, 2>), dim3(blocks), dim3(256), 0, st, t);
+        }
         for (int i = 0; i < n; ++i) { f16 *s = xt[i]; xt[i] = xt_next[i]; xt_next[i] = s; }
     }
 }

@@ -111,9 +111,10 @@ __device__ void sm_gram(const SmMat &p, const MuStep &s, int piece, float (*tile
 }
 __global__ __launch_bounds__(256) void mu_small_gram_kernel(SmTable t) {
     __shared__ float tile[kSmRows][kSmGramStride];
-    const int q = mu_which(t.f, blockIdx.x);
-    const SmMat &p = t.a[q];
-    const int piece = blockIdx.x - t.f.first[q];
+    SmMat p;
+    unsigned start;
+    mu_which(t.f, t.a, blockIdx.x, p, start);
+    const int piece = blockIdx.x - start;
     if (p.mt == 1) sm_gram<1>(p, t.s, piece, tile);
     else if (p.mt == 2) sm_gram<2>(p, t.s, piece, tile);
     else sm_gram<4>(p, t.s, piece, tile);
@@ -302,10 +303,11 @@ __device__ void sm_apply(const SmMat &p, const float *u, int n0, double *P, floa
 __global__ __launch_bounds__(256) void mu_small_apply_kernel(SmTable t) {
     __shared__ double P[64 * 66];
     __shared__ float tile[kSmRows][kSmApplyStride];
-    const int q = mu_which(t.f, blockIdx.x);
-    const SmMat &p = t.a[q];
+    SmMat p;
+    unsigned start;
+    mu_which(t.f, t.a, blockIdx.x, p, start);
     const float *u = p.u ? p.u : p.j.mom ? p.j.mom_out : p.j.grad;
-    const int n0 = (blockIdx.x - t.f.first[q]) * kSmRows;
+    const int n0 = (blockIdx.x - start) * kSmRows;
     if (p.mt == 1) sm_apply<1>(p, u, n0, P, tile);
     else if (p.mt == 2) sm_apply<2>(p, u, n0, P, tile);
     else sm_apply<4>(p, u, n0, P, tile);
