@@ -28,6 +28,7 @@ typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float mu_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int mu_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMuPad = 128;
@@ -50,12 +51,12 @@ __device__ __forceinline__ void mu_split(float v, f16 &hi, f16 &lo) {
     lo = (f16)(v - (float)hi);
 }
 // eight values along k, the first at a multiple of 8, as one piece each of hi and lo
-__device__ __forceinline__ void mu_put8(f16 *o, size_t at, const float (&v)[8]) {
+__device__ __forceinline__ void mu_put8(gptr<f16> o, size_t at, const float (&v)[8]) {
     f16x8 hi, lo;
 #pragma unroll
     for (int i = 0; i < 8; ++i) { f16 h, l; mu_split(v[i], h, l); hi[i] = h; lo[i] = l; }
-    *reinterpret_cast<f16x8 *>(o + at) = hi;
-    *reinterpret_cast<f16x8 *>(o + at + 512) = lo;
+    *(gptr<f16x8>)(o + at) = hi;
+    *(gptr<f16x8>)(o + at + 512) = lo;
 }
 
 // ---- the product of one tile -------------------------------------------------------------------------------------
@@ -64,14 +65,15 @@ __device__ __forceinline__ void mu_put8(f16 *o, size_t at, const float (&v)[8]) 
 // first row block; sa / sb: halves from one row block to the next.
 template <int TA> constexpr int kMuStage = (2 * TA + 4) * 4096;      // bytes of a stage
 template <int TA>
-__device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, size_t sb, int steps, char *lds, f32x16 (&acc)[TA][2]) {
+__device__ __forceinline__ void mu_tile(gptr<const f16> a, size_t sa, gptr<const f16> b, size_t sb, int steps, char *lds, f32x16 (&acc)[TA][2]) {
+    constexpr int STAGE = kMuStage<TA>;
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     mu_u32x4 ga[2 * TA], gb[4];
     auto fetch = [&](int s) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i < 2 * TA) ga[i] = *reinterpret_cast<const mu_u32x4 *>(a + i * sa + (size_t)s * 2048 + t * 8);
-            gb[i] = *reinterpret_cast<const mu_u32x4 *>(b + i * sb + (size_t)s * 2048 + t * 8);
+            if (i < 2 * TA) ga[i] = *(gptr<const mu_u32x4>)(a + i * sa + (size_t)s * 2048 + t * 8);
+            gb[i] = *(gptr<const mu_u32x4>)(b + i * sb + (size_t)s * 2048 + t * 8);
         }
     };
     auto store = [&](char *buf) {
@@ -81,7 +83,7 @@ __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, s
             *reinterpret_cast<mu_u32x4 *>(buf + (2 * TA + i) * 4096 + t * 16) = gb[i];
         }
     };
-    f32x16 low[TA][2];                                       // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
+    f32x16 low[TA][2];                                      // hi lo + lo hi: 2^-11 of the sum, so their roundings do not count
 #pragma unroll
     for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -115,21 +117,23 @@ __device__ __forceinline__ void mu_tile(const f16 *a, size_t sa, const f16 *b, s
     };
     // Everything that a group of products needs was asked for one group earlier: operands of the second half of a stage are read from
     // LDS under the products of the first, those of the next stage's first half under the products of the second; global loads
-    // run a stage and a half ahead.  The barrier publishes LDS only and leaves them in flight.
+    // run a stage and a half ahead (two and a half: 250 registers, and no faster).  The barrier publishes LDS only and leaves them
+    // in flight.  No branch in the loop: past one the compiler waits for every load it has issued; the last two stages ask for
+    // the last step again, and nobody reads it.
+    const int last = steps - 1;
     fetch(0);
     store(lds);
     fetch(1);                                                // (steps >= 2)
     lds_barrier();
     read(f0, lds, 0);
     for (int s = 0; s < steps; ++s) {
-        char *cur = lds + (s & 1) * kMuStage<TA>, *nxt = lds + ((s + 1) & 1) * kMuStage<TA>;
-        const bool more = s + 1 < steps;
+        char *cur = lds + (s & 1) * STAGE, *nxt = lds + ((s + 1) & 1) * STAGE;
         read(f1, cur, 1);
         multiply(f0);
-        if (more) store(nxt);                                // (every wave has read the stage before last: the barrier below)
+        store(nxt);                                          // (every wave has read the stage before last: the barrier below)
         lds_barrier();
-        if (more) read(f0, nxt, 0);
-        if (s + 2 < steps) fetch(s + 2);
+        read(f0, nxt, 0);
+        fetch(s + 2 < steps ? s + 2 : last);
         multiply(f1);
     }
     lds_barrier();
@@ -165,10 +169,10 @@ __device__ __forceinline__ int mu_item(unsigned b, unsigned n) {
 
 // ---- momentum and norm -------------------------------------------------------------------------------------------
 struct MuPrep {
-    const float *grad, *mom;         // mom null: U = grad
-    float *mom_out, *u;              // u: where U goes when it is neither grad nor mom_out (Nesterov), else null
-    const float *dsigma, *dot, *sigma, *scale;
-    double *part;                    // [blocks]
+    MuPtr<const float> grad, mom;    // mom null: U = grad
+    MuPtr<float> mom_out, u;         // u: where U goes when it is neither grad nor mom_out (Nesterov), else null
+    MuPtr<const float> dsigma, dot, sigma, scale;
+    MuPtr<double> part;              // [blocks]
     long n;
     int vec;
     unsigned blocks;
@@ -204,14 +208,14 @@ __global__ __launch_bounds__(256) void mu_prep_kernel(MuPrepTable t) {
         const long n4 = p.n >> 2;
         constexpr int U = 4;
         for (long i0 = (long)b * 256 + threadIdx.x; i0 < n4; i0 += (long)nb * 256 * U) {
-            float4 g[U], d[U], m[U];
+            mu_f4 g[U], d[U], m[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long i = i0 + (long)u * nb * 256;
                 if (i < n4) {
-                    g[u] = reinterpret_cast<const float4 *>(p.grad)[i];
-                    if (p.dsigma) d[u] = reinterpret_cast<const float4 *>(p.dsigma)[i];
-                    if (p.mom) m[u] = reinterpret_cast<const float4 *>(p.mom)[i];
+                    g[u] = p.grad.as<const mu_f4>()[i];
+                    if (p.dsigma) d[u] = p.dsigma.as<const mu_f4>()[i];
+                    if (p.mom) m[u] = p.mom.as<const mu_f4>()[i];
                 }
             }
 #pragma unroll
@@ -231,8 +235,8 @@ __global__ __launch_bounds__(256) void mu_prep_kernel(MuPrepTable t) {
                     ss += (double)gv[j] * (double)gv[j];
                 }
                 if (p.mom) {
-                    reinterpret_cast<float4 *>(p.mom_out)[i] = make_float4(mv[0], mv[1], mv[2], mv[3]);
-                    if (p.u) reinterpret_cast<float4 *>(p.u)[i] = make_float4(gv[0], gv[1], gv[2], gv[3]);
+                    p.mom_out.as<mu_f4>()[i] = mu_f4{mv[0], mv[1], mv[2], mv[3]};
+                    if (p.u) p.u.as<mu_f4>()[i] = mu_f4{gv[0], gv[1], gv[2], gv[3]};
                 }
             }
         }
@@ -247,10 +251,10 @@ __global__ __launch_bounds__(256) void mu_prep_kernel(MuPrepTable t) {
 
 // ---- X = U / ||U|| as packed [m, n] and [n, m] --------------------------------------------------------------------
 struct MuSplit {
-    const float *u;                  // [rows, cols]
-    const double *part;
+    MuPtr<const float> u;            // [rows, cols]
+    MuPtr<const double> part;
     int nparts;
-    f16 *x, *xt;                     // [mp, np] and [np, mp]
+    MuPtr<f16> x, xt;                     // [mp, np] and [np, mp]
     int rows, cols, mp, np, tall;    // tall: rows = n
 };
 struct MuSplitTable { MuFirst<kMuGroup> f; MuSplit j[kMuGroup]; };
@@ -284,7 +288,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuSplitTable t) {
     for (int i = 0; i < kMuPrepMax / 256; ++i) ss += (int)threadIdx.x + 256 * i < p.nparts ? d[i] : 0.0;
     ss = wave_sum(ss);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = ss;
-    f16 *nat = p.tall ? p.xt : p.x, *tra = p.tall ? p.x : p.xt;
+    const gptr<f16> nat = p.tall ? p.xt : p.x, tra = p.tall ? p.x : p.xt;
     __syncthreads();
     {
         const double s = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
@@ -311,9 +315,9 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuSplitTable t) {
 
 // ---- Gram matrix A = X X^T: one triangle of 128 x 128 tiles, the reduction over n split ----------------------------
 struct MuGram {
-    const f16 *x;
-    float *slab;                     // [splits][tiles][128][128]
-    f16 *a;                          // [mp, mp]
+    MuPtr<const f16> x;
+    MuPtr<float> slab;               // [splits][tiles][128][128]
+    MuPtr<f16> a;                    // [mp, mp]
     int mp, np, tiles, splits, steps_per;
 };
 struct MuGramTable { MuFirst<kMuGroup> f, r; MuGram j[kMuGroup]; };
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void mu_gram_kernel(MuGramTable t) {
     f32x16 acc[2][2];
     const size_t sx = mu_strip(p.np / 16);
     mu_tile<2>(p.x + (size_t)ti * 4 * sx + (size_t)s0 * 2048, sx, p.x + (size_t)tj * 4 * sx + (size_t)s0 * 2048, sx, steps, lds, acc);
-    float *o = p.slab + ((size_t)split * p.tiles + tile) * 128 * 128;
+    const gptr<float> o = p.slab + ((size_t)split * p.tiles + tile) * 128 * 128;
     const int w = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -355,13 +359,13 @@ __global__ __launch_bounds__(256) void mu_gram_reduce_kernel(MuGramTable t) {
     mu_tri(tile, ti, tj);
     const int r0 = (sub >> 2) * 32, c0 = (sub & 3) * 32, tc = (threadIdx.x & 7) * 4, tr = threadIdx.x >> 3;
     const double k = (double)kScaleA / ((double)kScaleX * kScaleX);
-    const float *s = p.slab + (size_t)tile * 128 * 128 + (r0 + tr) * 128 + c0 + tc;
+    const gptr<const float> s = p.slab + (size_t)tile * 128 * 128 + (r0 + tr) * 128 + c0 + tc;
     const size_t next = (size_t)p.tiles * 128 * 128;
     double v[4] = {0.0, 0.0, 0.0, 0.0};                      // (the splits' own sums are short: the long one is formed here)
     for (int z0 = 0; z0 < p.splits; z0 += 8) {
-        float4 f[8];
+        mu_f4 f[8];
 #pragma unroll
-        for (int z = 0; z < 8; ++z) f[z] = *reinterpret_cast<const float4 *>(s + (size_t)(z0 + z < p.splits ? z0 + z : z0) * next);
+        for (int z = 0; z < 8; ++z) f[z] = *(gptr<const mu_f4>)(s + (size_t)(z0 + z < p.splits ? z0 + z : z0) * next);
 #pragma unroll
         for (int z = 0; z < 8; ++z)
             if (z0 + z < p.splits) { v[0] += f[z].x; v[1] += f[z].y; v[2] += f[z].z; v[3] += f[z].w; }
@@ -385,9 +389,9 @@ __global__ __launch_bounds__(256) void mu_gram_reduce_kernel(MuGramTable t) {
 
 // ---- m x m products of commuting symmetric matrices: one triangle of tiles --------------------------------
 struct MuSquare {
-    const f16 *a, *b;                // o = alpha a b  (packed, symmetric, [mp, mp])
-    f16 *o;
-    const f16 *z;                    // polynomial form: o += zscale * z + diag on the diagonal; null: the plain product
+    MuPtr<const f16> a, b;           // o = alpha a b  (packed, symmetric, [mp, mp])
+    MuPtr<f16> o;
+    MuPtr<const f16> z;              // polynomial form: o += zscale * z + diag on the diagonal; null: the plain product
     float alpha, zscale, diag;
     int mp, tiles;
 };
@@ -426,15 +430,15 @@ __global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
     mu_tri_blocked(item, p.mp / 32, ti, tj);
     const int kb = p.mp / 16, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const size_t sr = mu_strip(kb);
-    const f16 *a = p.a + ti * sr + lane * 8, *b = p.b + tj * sr + lane * 8;
+    const gptr<const f16> a = p.a + ti * sr + lane * 8, b = p.b + tj * sr + lane * 8;
     struct Step { f16x8 a[2][2], b[2][2]; } f[kMuAhead];     // [ks][hi, lo]
     auto fetch = [&](int s, Step &x) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                x.a[ks][h] = *reinterpret_cast<const f16x8 *>(a + (size_t)s * 2048 + ks * 1024 + h * 512);
-                x.b[ks][h] = *reinterpret_cast<const f16x8 *>(b + (size_t)s * 2048 + ks * 1024 + h * 512);
+                x.a[ks][h] = *(gptr<const f16x8>)(a + (size_t)s * 2048 + ks * 1024 + h * 512);
+                x.b[ks][h] = *(gptr<const f16x8>)(b + (size_t)s * 2048 + ks * 1024 + h * 512);
             }
     };
     const int steps = p.mp / 128;                            // of this wave: w, w + 4, ...
@@ -447,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
     const int r = lane & 31, k = (w & 1) * 16 + (lane >> 5) * 8, R = (mirror ? tj : ti) * 32 + r, K = (mirror ? ti : tj) * 32 + k;
     const size_t o = mu_off(R, K, kb);
     f16x8 zh, zl;
-    if (p.z) { zh = *reinterpret_cast<const f16x8 *>(p.z + o); zl = *reinterpret_cast<const f16x8 *>(p.z + o + 512); }
+    if (p.z) { zh = *(gptr<const f16x8>)(p.z + o); zl = *(gptr<const f16x8>)(p.z + o + 512); }
     f32x16 acc = {}, low = {};
     for (int s0 = 0; s0 < steps; s0 += kMuAhead) {
 #pragma unroll
@@ -473,20 +477,20 @@ __global__ __launch_bounds__(256, 2) void mu_square_kernel(MuSquareTable t) {
     for (int e = 0; e < 8; ++e) {
         const int at = mirror ? mu_lds32(k + e, r) : mu_lds32(r, k) + e;
         v[e] = p.alpha * ((part[0][at] + part[1][at]) + (part[2][at] + part[3][at]));
-        if (p.z) {
-            v[e] += p.zscale * ((float)zh[e] + (float)zl[e]);
-            if (R == K + e) v[e] += p.diag;
-        }
+    }
+    if (p.z) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p.zscale * ((float)zh[e] + (float)zl[e]) + (R == K + e ? p.diag : 0.f);
     }
     mu_put8(p.o, o, v);
 }
 
 // ---- X <- P X, between two chains (packed, both layouts) or as the result ------------------------------------------
 struct MuApply {
-    const f16 *a, *b;                // tile rows from a, tile columns from b, reduction over mp
-    f16 *x, *xt;                     // not last: packed [mp, np], [np, mp]
-    const float *param;              // last, update form: out = keep * param - step * O; null: out = O
-    float *out;                      // last: [rows, cols]
+    MuPtr<const f16> a, b;           // tile rows from a, tile columns from b, reduction over mp
+    MuPtr<f16> x, xt;                // not last: packed [mp, np], [np, mp]
+    MuPtr<const float> param;        // last, update form: out = keep * param - step * O; null: out = O
+    MuPtr<float> out;                // last: [rows, cols]
     float alpha, keep, step;
     int mp, np, rows, cols, tiles_m, items, flip;
 };
@@ -630,7 +634,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
             p.dsigma = jobs[i].dsigma; p.dot = jobs[i].dot; p.sigma = jobs[i].sigma; p.scale = jobs[i].scale;
             p.part = (double *)(ws + m[i].part);
             p.n = (long)jobs[i].rows * jobs[i].cols;
-            p.vec = mu_aligned(p.grad) && mu_aligned(p.mom) && mu_aligned(p.mom_out) && mu_aligned(p.dsigma);
+            p.vec = mu_aligned(p.grad.p) && mu_aligned(p.mom.p) && mu_aligned(p.mom_out.p) && mu_aligned(p.dsigma.p);
             p.blocks = m[i].nparts;
             t.f.first[i] = blocks;
             blocks += m[i].nparts;
@@ -644,7 +648,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
         unsigned blocks = 0;
         for (int i = 0; i < n; ++i) {
             MuSplit &p = t.j[i];
-            p.u = keep_u ? (const float *)(ws + m[i].u) : update ? jobs[i].mom_out : jobs[i].grad;
+            p.u = keep_u ? (const float *)(ws + m[i].u) : update ? jobs[i].mom_out.p : jobs[i].grad.p;
             p.part = (const double *)(ws + m[i].part); p.nparts = m[i].nparts;
             x[i] = (f16 *)(ws + m[i].x); xt[i] = (f16 *)(ws + m[i].xt); xt_next[i] = (f16 *)(ws + m[i].xt2);
             p.x = x[i]; p.xt = xt[i];
@@ -731,7 +735,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
             p.tiles_m = flip ? m[i].mp / 128 : m[i].mp / (64 * ta);
             p.alpha = done == steps ? 1.f / (s_p * kScaleX) : 1.f / s_p;
             p.x = x[i]; p.xt = xt_next[i];
-            p.param = update ? jobs[i].param : nullptr; p.out = jobs[i].out; p.keep = jobs[i].keep; p.step = jobs[i].step;
+            p.param = update ? jobs[i].param.p : nullptr; p.out = jobs[i].out; p.keep = jobs[i].keep; p.step = jobs[i].step;
             t.f.first[i] = blocks;
             p.items = m[i].mp / 128 * (m[i].np / 128) * (2 / ta);
             blocks += (unsigned)(p.items + 7) & ~7u;

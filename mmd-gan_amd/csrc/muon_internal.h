@@ -7,11 +7,21 @@ namespace mmdgan {
 constexpr int kMuGroup = 16;                 // matrices per launch (the task tables travel by value)
 constexpr float kMuA = 3.4445f, kMuB = -4.7750f, kMuC = 2.0315f;
 
+// A pointer in a job.  Taken from a table by an index that is not a constant, a pointer may point anywhere as far as the compiler knows
+// and is read through flat accesses, which count as LDS traffic too: every LDS wait would wait for them.
+template <typename T> using gptr = __attribute__((address_space(1))) T *;
+template <typename T> struct MuPtr {
+    T *p;
+    MuPtr &operator=(T *q) { p = q; return *this; }
+    __device__ __forceinline__ operator gptr<T>() const { return (gptr<T>)p; }
+    template <typename U> __device__ __forceinline__ gptr<U> as() const { return (gptr<U>)(gptr<T>)p; }
+};
+
 struct MuJob {
     int rows, cols;
-    const float *grad, *mom, *param;         // mom, param null: orthogonalize
-    float *mom_out, *out;
-    const float *dsigma, *dot, *sigma, *scale;
+    MuPtr<const float> grad, mom, param;     // mom, param null: orthogonalize
+    MuPtr<float> mom_out, out;
+    MuPtr<const float> dsigma, dot, sigma, scale;
     float keep, step;                        // out = keep * param - step * O
 };
 struct MuStep { float momentum, grad_scale; int nesterov, steps; };

@@ -22,8 +22,8 @@ constexpr int kSmGramStride = 80, kSmApplyStride = 68;   // floats: conflict-fre
 
 struct SmMat {
     MuJob j;
-    float *u;                        // U where it is neither grad nor mom_out
-    double *slab, *p;                // [pieces][tiles][256]; [R][R]
+    MuPtr<float> u;                  // U where it is neither grad nor mom_out
+    MuPtr<double> slab, p;                // [pieces][tiles][256]; [R][R]
     int m, n, mt, pieces, per;       // mt 16-wide tiles; per: rows of n in a piece (a multiple of kSmRows)
 };
 struct SmTable { MuFirst<kMuGroup> f; SmMat a[kMuGroup]; MuStep s; };
@@ -106,7 +106,7 @@ __device__ void sm_gram(const SmMat &p, const MuStep &s, int piece, float (*tile
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int q = w + 4 * i;
-        if (q < NT) *reinterpret_cast<d4 *>(p.slab + ((size_t)piece * NT + q) * 256 + lane * 4) = acc[i];
+        if (q < NT) *(gptr<d4>)(p.slab + ((size_t)piece * NT + q) * 256 + lane * 4) = acc[i];
     }
 }
 __global__ __launch_bounds__(256) void mu_small_gram_kernel(SmTable t) {
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(1024) void mu_small_chain_kernel(SmTable t) {
 }
 
 template <int MT>
-__device__ void sm_apply(const SmMat &p, const float *u, int n0, double *P, float (*tile)[kSmApplyStride]) {
+__device__ void sm_apply(const SmMat &p, gptr<const float> u, int n0, double *P, float (*tile)[kSmApplyStride]) {
     constexpr int R = 16 * MT, ST = R + 2, L = MT * 4;
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const bool tall = p.j.rows >= p.j.cols;
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256) void mu_small_apply_kernel(SmTable t) {
     SmMat p;
     unsigned start;
     mu_which(t.f, t.a, blockIdx.x, p, start);
-    const float *u = p.u ? p.u : p.j.mom ? p.j.mom_out : p.j.grad;
+    const gptr<const float> u = p.u ? p.u.as<const float>() : p.j.mom ? p.j.mom_out.as<const float>() : (gptr<const float>)p.j.grad;
     const int n0 = (blockIdx.x - start) * kSmRows;
     if (p.mt == 1) sm_apply<1>(p, u, n0, P, tile);
     else if (p.mt == 2) sm_apply<2>(p, u, n0, P, tile);
@@ -339,7 +339,7 @@ void mu_small_run(const MuJob *jobs, int n, const MuStep &s, char *ws, hipStream
     unsigned gram = 0, apply = 0, first_apply[kMuGroup] = {};
     int widest = 1;
     for (int i = 0; i < n; ++i) {
-        const bool keep_u = jobs[i].mom && s.nesterov;
+        const bool keep_u = jobs[i].mom.p && s.nesterov;
         const SmPlace pl = sm_place(jobs[i].rows, jobs[i].cols, keep_u, at);
         at = pl.end;
         SmMat &p = t.a[i];

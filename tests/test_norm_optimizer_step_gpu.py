@@ -73,10 +73,13 @@ def test_step_with_group_norm_matches_the_oracle(make, mode):
     (1e-4 of a tensor in L2; the losses' floor of 4e-7 of their kernel means).  lrelu and tanh: no activation whose derivative
     a rounding could switch off entirely.
     What a loss may be off by has two parts.  |L - ref| <= |L - L64(s)| + |L64(s) - L64(s_ref)| with s the engine's scores, L64 the loss in
-    64 bits: the first is the loss kernel's, held to the bar above; the second is what scores that are right to fp32 make of a loss
-    that amplifies them.  The kernels here are exp(-d^2 / 2) with means of 5e-4, so d^2 / 2 is about 8 and a relative error e of the
-    distances is one of 16 e in every mean; the loss is a difference of means 15 times as large: 240 e, 1e-4 already at e = 4e-7 = 7 *
-    2^-24, less than ten layers of sums of up to 512 fp32 terms leave (sqrt(512) roundings each, 1.4e-6; ten in quadrature 4e-6).  So s itself is held in L2, and L64(s) to 240 * 4e-6 = 1e-3."""
+    64 bits: the first is the loss kernel's, the second what scores that are right to fp32 make of a loss that amplifies them.
+    First: the kernel forms d^2 = |x|^2 + |y|^2 - 2 x y from sums of 16 fp32 products, each off by 16 * 2^-24 of its terms at most, and adds
+    them with two more roundings: off by 18 * 2^-24 * (|x|^2 + |y|^2); exp(-d^2 / 2) by half of that relatively, 18 * 2^-24 * max |s|^2.  (The
+    4e-7 of the other tests is for scores of norm 1: here d^2 is about 16, the kernel means being 5e-4.)
+    Second: d^2 / 2 about 8, a relative error e of the distances is one of 16 e in every mean; the loss is a difference of means 15 times
+    as large: 240 e.  Ten layers of sums of up to 512 fp32 terms leave e = 4e-6 (sqrt(512) roundings each, in quadrature), the loss
+    1e-3.  The scores themselves are held in L2."""
     arch, B = make(), 8
     eng = engine(arch, B, launch_mode=mode)
     ora = R.OracleGan(arch, 'rep', (5e-4, 2e-4), dtype=torch.float64, params=eng.get_variables())
@@ -104,7 +107,7 @@ def test_step_with_group_norm_matches_the_oracle(make, mode):
         assert (s - s64).norm() <= 1e-4 * s64.norm(), step
         own = R.gan_loss(s[B:], s[:B], 'rep', B, rep_weights=eng.rep_weights)
         for i, (ref, mine) in enumerate(zip((float(lg), float(ld)), own)):
-            bar = 4e-7 * float(max(got[2:5]))
+            bar = (4e-7 + 18 * 2.0 ** -24 * float((s * s).sum(1).max())) * float(max(got[2:5]))
             assert abs(got[i] - float(mine)) <= 1e-4 * abs(float(mine)) + bar, (step, i, got[i], float(mine))
             assert abs(float(mine) - ref) <= 1e-3 * abs(ref) + bar, (step, i, float(mine), ref)
         if step == 0:
