@@ -8,8 +8,8 @@
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.  What the kernels do about it:
 //   gn_resident   one workgroup holds an image's channel slab (whole groups, all pixels) in registers between the sums and
-//                 the apply, so every tensor moves once.  Needs D a power of two and a slab of at most 256 KB (forward) /
-//                 128 KB per tensor (backward; with tanh 64 KB).
+//                 the apply, so every tensor moves once.  Needs C a multiple of 4, groups of a power of two up to 256 channels or of any
+//                 number up to 64, and a slab of at most 256 KB (forward) / 128 KB per tensor (backward; with tanh 64 KB).
 //   gn_partial + gn_apply   everything else: pixel chunks' sums to the workspace, then the apply pass reads x (and dy) again.
 // All arithmetic on elements is in 64 bits: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for memory
 // either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
@@ -23,6 +23,8 @@ constexpr int kGnMaxThreads = 512;                   // 256 VGPRs per wave: at m
 // 78 us, in two passes it takes 48; and 64x8x8x512 23 us where half of the registers had to do, now 13)
 constexpr int kGnFwdRegs = 32;
 template <bool TANH> constexpr int kGnBwdRegs = TANH ? 8 : 16;
+// ... and for slabs and groups that are no powers of two: half of it, 8 at most (ANY below)
+constexpr int gn_any_regs(int regs) { return regs / 2 < 8 ? regs / 2 : 8; }
 constexpr int kGnGrid = 1024;                        // workgroups of a launch: four per CU
 constexpr int kGnSplitCh = 256;                      // channels of a slab in the two-pass form
 
@@ -64,18 +66,22 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 // sums are of dz and dz x, sum dz xhat = rstd (sum dz x - mean sum dz).
 // GP: groups that a thread's four channels can belong to - 1 if D is a multiple of 4 (fewer registers, and the forward sums of the
 // four are one), else 4.  An item of the reduction is a channel, or (forward, GP = 1) a column of four.
-// red: [row groups][NV][CV] doubles, chan: [2][S] (backward totals of this workgroup), stat: [2][S].
-template <int U, bool BWD, bool TANH, int GP>
+// ANY: slabs and groups that are no powers of two - columns dealt to the threads by division, those that are left over idle, sums
+// through LDS from every thread instead of by shuffles.  64x8x8x320 in groups of 10: forward 7.8 us, backward 12.1 (in two passes 21.8 and
+// 30.9), 64x32x32x96 in groups of 3: 15.7 and 27.7 (16.7 and 31.6); with 16 float4 per thread and more the two passes win
+// (33x47x31x96: forward 14.8 us against 21.3), with tanh's code in the backward from 8 on (64x16x16x192: 20.0 against 26.9).
+// red: [row groups][NV][CV] doubles (ANY: [NV][T]), chan: [2][S] (backward totals of this workgroup), stat: [2][S].
+template <int U, bool BWD, bool TANH, int GP, bool ANY>
 __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
     constexpr bool kByCol = !BWD && GP == 1;
     constexpr int NV = kByCol ? 2 : 8;
     extern __shared__ double gn_lds[];
     const int T = blockDim.x, t = threadIdx.x, lane = t & 63;
     const int S = a.S, CV = S >> 2, RT = T / CV, D = a.D, HW = a.HW;
-    const int col = t & (CV - 1), row0 = t / CV;
+    const int col = ANY ? t % CV : t & (CV - 1), row0 = !ANY || t < RT * CV ? t / CV : HW;
     const int wide = CV < 64 ? 64 : CV, RG = T / wide, rg = t / wide;
     double *red = gn_lds;
-    double *chan = red + RG * NV * CV;
+    double *chan = red + (ANY ? T * NV : RG * NV * CV);
     double *stat = chan + 2 * S;
     // the slabs of an image share its cache lines: all of them on one XCD (workgroups go to the eight XCDs in turn, each has its
     // own L2) and close in time - groups of 8 images, image fastest
@@ -84,7 +90,9 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
     const int slab = in / wide_rows, row = group * 8 + in % wide_rows;
     const int c0 = slab * S + col * 4, g0 = slab * S / D, gps = S / D;
     const int items = kByCol ? CV : S, per_group = kByCol ? D >> 2 : D;      // items, and items per group
-    const int DW = per_group < 64 ? per_group : 64;    // neighbours that one wave reduces by shuffles
+    const int DW = ANY ? 1 : per_group < 64 ? per_group : 64;        // neighbours that one wave reduces by shuffles
+    int LN = 64;                                       // ANY: lanes that share an item
+    while (LN > 1 && S * LN > T) LN >>= 1;
     const int per = per_group / DW;
     const float4 gv = *reinterpret_cast<const float4 *>(a.gamma + c0), bv = *reinterpret_cast<const float4 *>(a.beta + c0);
     const float ga[4] = {gv.x, gv.y, gv.z, gv.w}, be[4] = {bv.x, bv.y, bv.z, bv.w};
@@ -138,22 +146,39 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
             if (BWD && TANH) vd[u] = make_float4(dv[0], dv[1], dv[2], dv[3]);
         }
         // lanes of a wave that hold the same column
-        for (int o = 32; o >= CV; o >>= 1) {
+        if (!ANY) {
+            for (int o = 32; o >= CV; o >>= 1) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) s[k] += __shfl_xor(s[k], o, 64);
+                for (int k = 0; k < NV; ++k) s[k] += __shfl_xor(s[k], o, 64);
+            }
         }
-        if (CV >= 64 || lane < CV) {
+        if (ANY) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) red[k * T + t] = s[k];
+        } else if (CV >= 64 || lane < CV) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) red[(rg * NV + k) * CV + col] = s[k];
         }
         __syncthreads();
         // totals over the row groups, then over the group's items
-        for (int i = t; i < items; i += T) {
+        for (int i0 = 0; i0 < (ANY ? S : items); i0 += ANY ? T / LN : T) {
+            const int i = i0 + (ANY ? t / LN : t);
+            if (!ANY && i >= items) break;
             const int k = kByCol ? 0 : i & 3, q = kByCol ? i : i >> 2;
             double s1 = 0.0, s2 = 0.0;
-            for (int z = 0; z < RG; ++z) {
-                s1 += red[(z * NV + k) * CV + q];
-                s2 += red[(z * NV + (kByCol ? 1 : 4) + k) * CV + q];
+            if (ANY) {
+                if (i < S)
+                    for (int z = t & (LN - 1); z < RT; z += LN) {
+                        s1 += red[k * T + z * CV + q];
+                        s2 += red[(4 + k) * T + z * CV + q];
+                    }
+                for (int o = LN >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+                if (i >= S || (t & (LN - 1))) continue;
+            } else {
+                for (int z = 0; z < RG; ++z) {
+                    s1 += red[(z * NV + k) * CV + q];
+                    s2 += red[(z * NV + (kByCol ? 1 : 4) + k) * CV + q];
+                }
             }
             if (BWD) {
                 const double *st = a.stats + 2 * ((size_t)ns * a.G + (slab * S + i) / D);
@@ -170,6 +195,11 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
 #pragma unroll
         for (int j = 0; j < GP; ++j) {
             const int g = (col * 4 + j) / D;
+            if (ANY && j && g == (col * 4 + j - 1) / D) {    // (the same group as the channel before)
+                mean[j] = mean[j ? j - 1 : 0]; rstd[j] = rstd[j ? j - 1 : 0];
+                if (BWD) { L[j] = L[j ? j - 1 : 0]; M[j] = M[j ? j - 1 : 0]; }
+                continue;
+            }
             double s1 = 0.0, s2 = 0.0;
             for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
             s1 *= inv_m; s2 *= inv_m;
@@ -216,7 +246,8 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
         if (n + a.rows < a.N) __syncthreads();         // red and stat are written again for the next image
     }
     if (BWD && a.part) {
-        for (int i = t; i < S; i += T) {               // (the thread that owns item i wrote chan[i])
+        if (ANY) __syncthreads();
+        for (int i = t; i < S; i += T) {               // (else the thread that owns item i wrote chan[i])
             double *p = a.part + (size_t)row * 2 * a.C + slab * S + i;
             p[0] = chan[i]; p[a.C] = chan[S + i];
         }
@@ -451,14 +482,32 @@ static inline bool gn_pow2(long v) { return v > 0 && (v & (v - 1)) == 0; }
 // How a geometry runs; the same for the workspace query and for the call (which may still fall back from the resident form
 // when a pointer is not 16-byte aligned: the workspace covers both).
 struct GnPlan {
-    bool resident;
+    bool resident, any;
     int S, T, U;                 // resident: slab channels, threads, float4 per thread
     int SB, gps, pieces, slabs, chunks, chunk_px;     // two-pass
 };
 // regs: float4 per thread and tensor at most
 static void gn_plan_resident(long HW, int C, int D, long N, int regs, GnPlan &p) {
     p.resident = false;
-    if ((C & 3) || !gn_pow2(D) || D > kGnSplitCh) return;
+    p.any = !gn_pow2(D);
+    if ((C & 3) || D > (p.any ? 64 : kGnSplitCh)) return;
+    if (p.any) {
+        regs = gn_any_regs(regs);
+        // whole groups and whole float4: multiples of `unit`, the widest of at most 64 channels that occupies the CUs and fits
+        const int unit = D % 4 == 0 ? D : D % 2 == 0 ? 2 * D : 4 * D;
+        int best = 0;
+        for (int S = unit; S <= C && (S == unit || S <= 64); S += unit) {
+            if (C % S) continue;
+            long T = 64, U = 1;
+            while (T < kGnMaxThreads && T * 4 < HW * (S / 4)) T *= 2;
+            const long RT = T / (S / 4);
+            while (U * RT < HW && U <= regs) U *= 2;
+            if (U > regs || (best && N * (C / S) < 256)) continue;
+            best = S; p.S = S; p.T = (int)T; p.U = (int)U;
+        }
+        p.resident = best > 0;
+        return;
+    }
     int top = 4;                                       // widest power-of-two slab that divides C
     while (top < kGnSplitCh && C % (top * 2) == 0) top *= 2;
     if (top < D) return;
@@ -505,18 +554,19 @@ static size_t gn_bytes(long N, long HW, int C, int G) {
 
 static bool gn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-template <bool BWD, bool TANH, int GP>
+template <bool BWD, bool TANH, int GP, bool ANY>
 static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st) {
     const int CV = p.S / 4, wide = CV < 64 ? 64 : CV;
-    const size_t lds = ((size_t)(p.T / wide) * (!BWD && GP == 1 ? 2 : 8) * CV + 4 * (size_t)p.S) * sizeof(double);
+    const size_t lds = ((ANY ? (size_t)p.T * 8 : (size_t)(p.T / wide) * (!BWD && GP == 1 ? 2 : 8) * CV) + 4 * (size_t)p.S) * sizeof(double);
     const dim3 grid((unsigned)(a.rows * a.slabs)), block(p.T);
+    constexpr int REGS = BWD ? kGnBwdRegs<TANH> : kGnFwdRegs, MOST = ANY ? gn_any_regs(REGS) : REGS;      // U at most
     switch (p.U) {
-        case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case 8: hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case 16: if constexpr (!BWD || kGnBwdRegs<TANH> == 16) hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH, GP>), grid, block, lds, st, a); break;
-        case kGnFwdRegs: if constexpr (!BWD) hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, false, TANH, GP>), grid, block, lds, st, a); break;
+        case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
+        case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
+        case 4: hipLaunchKernelGGL((gn_resident_kernel<4, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
+        case 8: if constexpr (MOST >= 8) hipLaunchKernelGGL((gn_resident_kernel<8, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
+        case 16: if constexpr (MOST >= 16) hipLaunchKernelGGL((gn_resident_kernel<16, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
+        case kGnFwdRegs: if constexpr (MOST >= kGnFwdRegs) hipLaunchKernelGGL((gn_resident_kernel<kGnFwdRegs, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
     }
 }
 
@@ -533,8 +583,9 @@ static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipSt
         a.rows = (int)gn_resident_rows(a.N, a.slabs);
         part_rows = a.rows;
         a.part = params ? (double *)workspace : nullptr;
-        if (a.D % 4 == 0) gn_launch_resident<BWD, TANH, 1>(a, p, st);
-        else gn_launch_resident<BWD, TANH, 4>(a, p, st);
+        if (p.any) gn_launch_resident<BWD, TANH, 4, true>(a, p, st);
+        else if (a.D % 4 == 0) gn_launch_resident<BWD, TANH, 1, false>(a, p, st);
+        else gn_launch_resident<BWD, TANH, 4, false>(a, p, st);
     } else {
         gn_plan_split(a.HW, a.C, a.D, a.N, p);
         a.SB = p.SB; a.gps = p.gps; a.pieces = p.pieces; a.slabs = p.slabs; a.chunks = p.chunks; a.chunk_px = p.chunk_px;

@@ -89,6 +89,13 @@ def test_forward_and_backward_match_the_definition(ops, N, HW, C, G):
         assert ((dbeta.cpu().double() - rb).abs() <= U * rb.abs() + slack * a.sum(dim=(0, 1))).all()
 
 
+@pytest.mark.parametrize('N,HW,C,G', [(33, 1457, 96, 32), (5, 100, 48, 16), (3, 77, 20, 4), (2, 600, 160, 32), (300, 9, 60, 12), (1, 16, 252, 4), (2, 333, 192, 32),
+                                      (3, 200, 96, 8), (1100, 3, 12, 4), (2, 2900, 12, 4), (1, 1, 12, 4), (2, 40, 240, 4), (2, 700, 252, 4), (1, 5000, 12, 4)])
+def test_groups_that_are_no_power_of_two(ops, N, HW, C, G):
+    """3, 5, 6, 12, 60, 63 channels a group, from one pixel to more than a workgroup keeps, more images than workgroups"""
+    test_forward_and_backward_match_the_definition(ops, N, HW, C, G)
+
+
 @pytest.mark.parametrize('N,HW,C,G,act', [(3, 40, 32, 8, 'tanh'), (2, 33, 15, 5, 'tanh'), (2, 2100, 64, 2, 'linear')])
 def test_gradient_against_differences(ops, N, HW, C, G, act):
     """<dx, v> against the central difference of sum(y dy) along v, in 64 bits: O(h^2) with h = 1e-4 and derivatives of a few
