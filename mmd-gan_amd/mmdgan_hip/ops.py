@@ -511,7 +511,7 @@ def _gn_ws(workspace, N, HW, C, G, device):
     need = _lib.load().mmdgan_gn_workspace_bytes(N, HW, C, G)
     if workspace is None:
         return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
-    assert workspace.is_cuda and workspace.numel() * workspace.element_size() >= need, \
+    assert workspace.is_cuda and workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need, \
         'group_norm: the workspace holds {} bytes, {} are needed'.format(workspace.numel() * workspace.element_size(), need)
     return workspace
 
@@ -885,7 +885,7 @@ def _muon_ws(jobs, steps, device, workspace=None):
             len(jobs), ', '.join('%dx%d' % (j.rows, j.cols) for j in jobs), steps))
     if workspace is None:
         return torch.empty(need, device=device, dtype=torch.uint8)
-    assert workspace.is_cuda and workspace.numel() * workspace.element_size() >= need, \
+    assert workspace.is_cuda and workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need, \
         'the workspace holds {} bytes, {} are needed'.format(workspace.numel() * workspace.element_size(), need)
     return workspace
 
@@ -921,7 +921,8 @@ class MuonGroup:
     """mmdgan_muon_update over a list of matrix parameters: momentum, orthogonalisation of the momentum matrix, weight decay and
     the step, all matrices together.  Vectors (biases, norms' gamma / beta) stay with AdamGroup / AdamArena.
     fixups: per parameter None or dict(dsigma=, dot=, sigma=, scale=) of device tensors, the spectral-norm fix-up applied as the
-    gradient is read (as AdamArena's segments).  out_params / out_momenta: where the results go (default: in place)."""
+    gradient is read (as AdamArena's segments).  out_params / out_momenta: where the results go (default: in place).
+    Pointers are taken once: the tensors stay where they are for the life of the group."""
 
     fold_fixup = True        # False: the caller applied sn_wgrad_fixup itself (data-parallel replicas, before their all-reduce)
 

@@ -273,3 +273,14 @@ def test_refusals_on_the_device(ops):
         ops.group_norm_bwd(x, torch.cat([dy, dy, dy]), gamma, beta, stats)
     with pytest.raises(ValueError, match='eps'):
         ops.group_norm_fwd(x, gamma, beta, 3, eps=0.0)
+
+
+def test_a_workspace_is_real_memory(ops):
+    """an expanded tensor counts more bytes than it has"""
+    x, v = torch.randn(2, 9, 12, device='cuda'), torch.ones(12, device='cuda')
+    fake = torch.zeros(1, device='cuda', dtype=torch.uint8).expand(1 << 20)
+    y, st = ops.group_norm_fwd(x, v, v, 3)
+    with pytest.raises(AssertionError, match='workspace'):
+        ops.group_norm_fwd(x, v, v, 3, workspace=fake)
+    with pytest.raises(AssertionError, match='workspace'):
+        ops.group_norm_bwd(x, x, v, v, st, workspace=fake)

@@ -294,3 +294,39 @@ def test_refusals_on_the_device(ops):
         ops.MuonGroup([u], [u.t().contiguous()], [u.clone()])
     with pytest.raises(AssertionError):
         ops.MuonGroup([], [], [])
+
+
+def test_workspaces_are_real_memory_and_outputs_apart(ops):
+    """an expanded tensor counts more bytes than it has; a parameter given twice would be updated by two workgroups at once"""
+    u, v = torch.randn(20, 30, device='cuda'), torch.randn(20, 30, device='cuda')
+    fake = torch.zeros(1, device='cuda', dtype=torch.uint8).expand(1 << 24)
+    with pytest.raises(AssertionError, match='workspace'):
+        ops.orthogonalize(u, workspace=fake)
+    g = ops.MuonGroup([u], [v], [torch.zeros_like(u)])
+    with pytest.raises(AssertionError, match='workspace'):
+        g.step(0.1, workspace=fake)
+    for call in (lambda: ops.orthogonalize([u, v], out=[v, u]), lambda: ops.orthogonalize([u, v], out=[u, u]),
+                 lambda: ops.MuonGroup([u, u], [v, v], [torch.zeros_like(u) for _ in range(2)]).step(0.1),
+                 lambda: ops.MuonGroup([u], [v], [v]).step(0.1)):
+        with pytest.raises(ValueError, match='overlaps'):
+            call()
+    a, b = ops.orthogonalize([u, u])                         # the same input twice is no conflict
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('shapes', [[(65 + i, 90 - i) for i in range(20)], [(900, 1300), (1024, 1200), (1281, 901), (300, 3000), (1000, 1100), (513, 2049)] * 2])
+def test_what_a_matrix_gets_does_not_depend_on_the_others(ops, shapes):
+    """more large matrices than a launch's table holds; enough of them for the larger tiles of the last product.  Every element is the
+    same sum in the same order: the bits of a call of its own"""
+    us = [make('gradient', r, c, i).cuda() for i, (r, c) in enumerate(shapes)]
+    together = ops.orthogonalize(us)
+    for u, o in zip(us, together):
+        assert torch.equal(ops.orthogonalize(u), o), u.shape
+    ref = orth64(us[1].cpu())
+    assert float((together[1].cpu().double() - ref).norm()) <= tolerance(us[1].cpu(), ref)
+    ps, ms = [torch.randn_like(u) for u in us], [torch.zeros_like(u) for u in us]
+    alone = [p.clone() for p in ps]
+    for p, u in zip(alone, us):
+        ops.MuonGroup([p], [u], [torch.zeros_like(u)]).step(0.1)
+    ops.MuonGroup(ps, us, ms).step(0.1)
+    assert all(torch.equal(p, q) for p, q in zip(ps, alone))
