@@ -83,11 +83,12 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
     double *red = gn_lds;
     double *chan = red + (ANY ? T * NV : RG * NV * CV);
     double *stat = chan + 2 * S;
-    // the slabs of an image share its cache lines: all of them on one XCD (workgroups go to the eight XCDs in turn, each has its
-    // own L2) and close in time - groups of 8 images, image fastest
+    // the slabs of an image share its cache lines: neighbours on one XCD (workgroups go to the eight XCDs in turn, each has its own
+    // L2) and close in time - of every 8 images, slab fastest, an XCD takes an eighth
     const int group = blockIdx.x / (8 * a.slabs), in = blockIdx.x - group * 8 * a.slabs;
-    const int wide_rows = a.rows - group * 8 < 8 ? a.rows - group * 8 : 8;
-    const int slab = in / wide_rows, row = group * 8 + in % wide_rows;
+    const int count = (a.rows - group * 8 < 8 ? a.rows - group * 8 : 8) * a.slabs, xcd = in & 7, rest = count & 7;
+    const int item = xcd * (count >> 3) + (xcd < rest ? xcd : rest) + (in >> 3);
+    const int slab = item % a.slabs, row = group * 8 + item / a.slabs;
     const int c0 = slab * S + col * 4, g0 = slab * S / D, gps = S / D;
     const int items = kByCol ? CV : S, per_group = kByCol ? D >> 2 : D;      // items, and items per group
     const int DW = ANY ? 1 : per_group < 64 ? per_group : 64;        // neighbours that one wave reduces by shuffles
