@@ -487,30 +487,36 @@ struct GnPlan {
     int S, T, U;                 // resident: slab channels, threads, float4 per thread
     int SB, gps, pieces, slabs, chunks, chunk_px;     // two-pass
 };
-// regs: float4 per thread and tensor at most
+// regs: float4 per thread and tensor at most.  ANY form: whole groups and whole float4, multiples of `unit`, the widest of at most 64
+// channels that occupies the CUs and fits.
+static void gn_plan_any(long HW, int C, int D, long N, int regs, GnPlan &p) {
+    const int unit = D % 4 == 0 ? D : D % 2 == 0 ? 2 * D : 4 * D, most = gn_any_regs(regs);
+    p.resident = false;
+    p.any = true;
+    if (D > 64) return;
+    for (int S = unit; S <= C && (S == unit || S <= 64); S += unit) {
+        if (C % S) continue;
+        long T = 64, U = 1;
+        while (T < kGnMaxThreads && T * 4 < HW * (S / 4)) T *= 2;
+        const long RT = T / (S / 4);
+        while (U * RT < HW && U <= most) U *= 2;
+        if (U > most || (p.resident && N * (C / S) < 256)) continue;
+        p.resident = true;
+        p.S = S; p.T = (int)T; p.U = (int)U;
+    }
+}
 static void gn_plan_resident(long HW, int C, int D, long N, int regs, GnPlan &p) {
     p.resident = false;
-    p.any = !gn_pow2(D);
-    if ((C & 3) || D > (p.any ? 64 : kGnSplitCh)) return;
-    if (p.any) {
-        regs = gn_any_regs(regs);
-        // whole groups and whole float4: multiples of `unit`, the widest of at most 64 channels that occupies the CUs and fits
-        const int unit = D % 4 == 0 ? D : D % 2 == 0 ? 2 * D : 4 * D;
-        int best = 0;
-        for (int S = unit; S <= C && (S == unit || S <= 64); S += unit) {
-            if (C % S) continue;
-            long T = 64, U = 1;
-            while (T < kGnMaxThreads && T * 4 < HW * (S / 4)) T *= 2;
-            const long RT = T / (S / 4);
-            while (U * RT < HW && U <= regs) U *= 2;
-            if (U > regs || (best && N * (C / S) < 256)) continue;
-            best = S; p.S = S; p.T = (int)T; p.U = (int)U;
-        }
-        p.resident = best > 0;
-        return;
-    }
+    if ((C & 3) || D > kGnSplitCh) return;
     int top = 4;                                       // widest power-of-two slab that divides C
     while (top < kGnSplitCh && C % (top * 2) == 0) top *= 2;
+    // ... of 4 or 8 channels reads 16 or 32 bytes of a pixel at a time: the other form's wider slabs first (64x16x16x200 in groups of one:
+    // forward 12.5 -> 10.2 us, backward 27.9 -> 19.2; with tanh's backward and 8 channels 20.8 -> 26.9, so not there)
+    if (!gn_pow2(D) || (top < (regs > 8 ? 16 : 8) && top < C)) {
+        gn_plan_any(HW, C, D, N, regs, p);
+        if (p.resident || !gn_pow2(D)) return;
+    }
+    p.any = false;
     if (top < D) return;
     const long cap = (long)kGnMaxThreads * regs;
     int least = D < 4 ? 4 : D;
