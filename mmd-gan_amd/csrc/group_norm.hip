@@ -69,7 +69,7 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 // ANY: slabs and groups that are no powers of two - columns dealt to the threads by division, those that are left over idle, sums
 // through LDS from every thread instead of by shuffles.  64x8x8x320 in groups of 10: forward 7.8 us, backward 12.1 (in two passes 21.8 and
 // 30.9), 64x32x32x96 in groups of 3: 15.7 and 27.7 (16.7 and 31.6); with 16 float4 per thread and more the two passes win
-// (33x47x31x96: forward 14.8 us against 21.3), with tanh's code in the backward from 8 on (64x16x16x192: 20.0 against 26.9).
+// (33x47x31x96: forward 14.0 us against 21.3), with tanh's code in the backward from 8 on (64x16x16x192: 20.0 against 26.9).
 // red: [row groups][NV][CV] doubles (ANY: [NV][T]), chan: [2][S] (backward totals of this workgroup), stat: [2][S].
 template <int U, bool BWD, bool TANH, int GP, bool ANY>
 __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
@@ -398,6 +398,19 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
             st[0] = mu; st[1] = is;
         }
     };
+    const int c = sl.c0 + col * VEC;
+    const float *px = a.x + (size_t)ns * a.HW * a.C + c;
+    const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
+    float vx[U][VEC], vd[BWD ? U : 1][VEC];
+    auto fetch = [&](int r) {                          // (a row beyond the chunk: its last row again, never used)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = r + u * RT < p1 ? r + u * RT : p1 - 1;
+            gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
+            if (BWD) gn_load<VEC>(pd + (size_t)rr * a.C, vd[BWD ? u : 0]);
+        }
+    };
+    fetch(p0 + rl);                                    // in flight while the statistics come together
     const int lanes = gn_lanes(sl.groups), mine = t / lanes, l = t & (lanes - 1);
     double u1 = 0.0, u2 = 0.0;
     if (mine < sl.groups) {
@@ -409,44 +422,34 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
     if (mine < sl.groups && l == 0) publish(mine, u1, u2);
     __syncthreads();
     if (rl >= RT) return;
-    const int c = sl.c0 + col * VEC;
-    double mean[VEC], rstd[VEC], m1[VEC], m2[VEC], ga[VEC], be[VEC];
+    double A[VEC], B[VEC], L[VEC], M[VEC];             // the maps of the resident form
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const int g = (c + j) / a.D - sl.g0;
-        ga[j] = a.gamma[c + j]; be[j] = a.beta[c + j];
+        double mean, rstd;
         if (BWD) {
             const double *st = a.stats + 2 * ((size_t)ns * a.G + sl.g0 + g);
-            mean[j] = st[0]; rstd[j] = st[1]; m1[j] = stat[0][g]; m2[j] = stat[1][g];
+            mean = st[0]; rstd = st[1];
+            L[j] = -rstd * rstd * stat[1][g];
+            M[j] = -fma(L[j], mean, rstd * stat[0][g]);
         } else {
-            mean[j] = stat[0][g]; rstd[j] = stat[1][g]; m1[j] = 0.0; m2[j] = 0.0;
+            mean = stat[0][g]; rstd = stat[1][g];
         }
+        A[j] = rstd * (double)a.gamma[c + j];
+        B[j] = fma(-mean, A[j], (double)a.beta[c + j]);
     }
-    const float *px = a.x + (size_t)ns * a.HW * a.C + c;
-    const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
     float *po = a.out + (size_t)n * a.HW * a.C + c;
     for (int r = p0 + rl; r < p1; r += RT * U) {
-        float vx[U][VEC], vd[U][VEC];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int rr = r + u * RT;
-            if (rr < p1) {
-                gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
-                if (BWD) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) { vx[u][j] = 0.f; vd[u][j] = 0.f; }
-            }
-        }
+        if (r != p0 + rl) fetch(r);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int rr = r + u * RT;
             float o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const double xh = ((double)vx[u][j] - mean[j]) * rstd[j], z = fma(xh, ga[j], be[j]);
+                const double v = vx[u][j], z = fma(A[j], v, B[j]);
                 if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
-                else o[j] = (float)(rstd[j] * (fma(ga[j], (double)vd[u][j] * gn_slope<TANH>(z, a.below), -m1[j]) - xh * m2[j]));
+                else o[j] = (float)fma(A[j], (double)vd[BWD ? u : 0][j] * gn_slope<TANH>(z, a.below), fma(L[j], v, M[j]));
             }
             if (rr < p1) {
                 if (VEC == 4) *reinterpret_cast<float4 *>(po + (size_t)rr * a.C) = make_float4(o[0], o[1 % VEC], o[2 % VEC], o[3 % VEC]);
