@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
     const int count = (a.rows - group * 8 < 8 ? a.rows - group * 8 : 8) * a.slabs, xcd = in & 7, rest = count & 7;
     const int item = xcd * (count >> 3) + (xcd < rest ? xcd : rest) + (in >> 3);
     const int slab = item % a.slabs, row = group * 8 + item / a.slabs;
-    const int c0 = slab * S + col * 4, g0 = slab * S / D, gps = S / D;
+    const int c0 = slab * S + col * 4, g0 = slab * S / D;
     const int items = kByCol ? CV : S, per_group = kByCol ? D >> 2 : D;      // items, and items per group
     const int DW = ANY ? 1 : per_group < 64 ? per_group : 64;        // neighbours that one wave reduces by shuffles
     int LN = 64;                                       // ANY: lanes that share an item
