@@ -41,12 +41,17 @@ __device__ __forceinline__ void sm_tri(int t, int &ti, int &tj) {
     tj = t - ti * (ti + 1) / 2;
 }
 
-// element e of rows [n0, n0 + kSmRows) of the [n, m] matrix: its index in memory (rows x cols), its place in the tile
-__device__ __forceinline__ bool sm_at(const SmMat &p, int n0, int e, size_t &at, int &r, int &c) {
+// element e of rows [n0, n0 + kSmRows) of the [n, m] matrix: its index in memory (rows x cols), its place in the tile.  inv_m = 1 / m: the
+// quotient is exact ((e + 1/2) / m is at least 1/128 from an integer, the product's error at most 2^-10 at e < 4096).
+__device__ __forceinline__ bool sm_at(const SmMat &p, int n0, int e, float inv_m, size_t &at, int &r, int &c) {
     const bool tall = p.j.rows >= p.j.cols;
-    if (tall) { r = e / p.m; c = e - r * p.m; at = (size_t)(n0 + r) * p.m + c; }
+    if (tall) { r = (int)(((float)e + 0.5f) * inv_m); c = e - r * p.m; at = (size_t)n0 * p.m + e; }
     else { c = e >> 6; r = e & 63; at = (size_t)c * p.n + n0 + r; }
     return n0 + r < p.n;
+}
+// columns beyond m of a tile: zero (four threads a row)
+template <int MT, int STRIDE> __device__ __forceinline__ void sm_clear(float (*tile)[STRIDE], int m) {
+    for (int c = m + (threadIdx.x & 3); c < 16 * MT; c += 4) tile[threadIdx.x >> 2][c] = 0.f;
 }
 
 template <int MT>
@@ -59,8 +64,8 @@ __device__ void sm_gram(const SmMat &p, const MuStep &s, int piece, float (*tile
     d4 acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = d4{0.0, 0.0, 0.0, 0.0};
-    for (int e = t; e < kSmRows * kSmGramStride; e += 256) (&tile[0][0])[e] = 0.f;           // columns beyond m stay zero
-    __syncthreads();
+    const float inv_m = 1.f / (float)p.m;
+    sm_clear<MT>(tile, p.m);                                 // (published with the first rows)
     for (int n0 = begin; n0 < end; n0 += kSmRows) {
         constexpr int L = MT * 4;                            // kSmRows * 16 MT / 256
         float g[L], d[L], m[L];
@@ -68,7 +73,7 @@ __device__ void sm_gram(const SmMat &p, const MuStep &s, int piece, float (*tile
         for (int i = 0; i < L; ++i) {
             const int e = t + 256 * i;
             size_t at; int r, c;
-            const bool ok = e < kSmRows * p.m && sm_at(p, n0, e, at, r, c);
+            const bool ok = e < kSmRows * p.m && sm_at(p, n0, e, inv_m, at, r, c);
             g[i] = ok ? p.j.grad[at] : 0.f;
             d[i] = ok && p.j.dsigma ? p.j.dsigma[at] : 0.f;
             m[i] = ok && p.j.mom ? p.j.mom[at] : 0.f;
@@ -78,7 +83,7 @@ __device__ void sm_gram(const SmMat &p, const MuStep &s, int piece, float (*tile
             const int e = t + 256 * i;
             size_t at; int r, c;
             if (e >= kSmRows * p.m) continue;
-            const bool ok = sm_at(p, n0, e, at, r, c);
+            const bool ok = sm_at(p, n0, e, inv_m, at, r, c);
             float u = c0 * g[i];
             if (p.j.dsigma) u -= c1 * d[i];
             if (p.j.mom) {
@@ -249,17 +254,18 @@ __device__ void sm_apply(const SmMat &p, gptr<const float> u, int n0, double *P,
     constexpr int R = 16 * MT, ST = R + 2, L = MT * 4;
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const bool tall = p.j.rows >= p.j.cols;
+    const float inv_m = 1.f / (float)p.m;
     float v[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
         const int e = t + 256 * i;
         size_t at; int r, c;
-        v[i] = e < kSmRows * p.m && sm_at(p, n0, e, at, r, c) ? u[at] : 0.f;
+        v[i] = e < kSmRows * p.m && sm_at(p, n0, e, inv_m, at, r, c) ? u[at] : 0.f;
     }
     double pv[R * R / 256];                                  // (every load of the workgroup in flight before the first is used)
 #pragma unroll
     for (int i = 0; i < R * R / 256; ++i) pv[i] = p.p[t + 256 * i];
-    for (int e = t; e < kSmRows * kSmApplyStride; e += 256) (&tile[0][0])[e] = 0.f;
+    sm_clear<MT>(tile, p.m);
     // this wave's 16 rows of n and all of m: (row, column) of the result in memory, its parameter before the products
     float old[MT][4];
     size_t at[MT][4];
@@ -275,12 +281,11 @@ __device__ void sm_apply(const SmMat &p, gptr<const float> u, int n0, double *P,
         }
 #pragma unroll
     for (int i = 0; i < R * R / 256; ++i) { const int e = t + 256 * i; P[e / R * ST + e % R] = pv[i]; }
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < L; ++i) {
         const int e = t + 256 * i;
         size_t a; int r, c;
-        if (e < kSmRows * p.m) { (void)sm_at(p, n0, e, a, r, c); tile[r][c] = v[i]; }
+        if (e < kSmRows * p.m) { (void)sm_at(p, n0, e, inv_m, a, r, c); tile[r][c] = v[i]; }
     }
     __syncthreads();
     d4 acc[MT];

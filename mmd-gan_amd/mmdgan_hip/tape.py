@@ -218,9 +218,9 @@ class _Net:
         c, groups = self.shapes[x][0], d['groups']
         if groups is None:
             groups = math.gcd(c, 32)
-        if not isinstance(groups, int) or groups < 1 or c % groups:
+        if not hasattr(groups, '__index__') or groups < 1 or c % groups:
             raise ValueError('{}: {} channels do not divide into {} groups'.format(scope, c, groups))
-        return self._emit('gn', [x], self.shapes[x], prefix=scope + '/GN' + suffix, act=act, groups=groups)
+        return self._emit('gn', [x], self.shapes[x], prefix=scope + '/GN' + suffix, act=act, groups=int(groups))
 
     def _scale(self, x, scale):                                          # ImageScaling, layer_func.py:1041-1176
         method, factor = scale
