@@ -9,7 +9,7 @@
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.  What the kernels do about it:
 //   gn_resident   one workgroup holds an image's channel slab (whole groups, all pixels) in registers between the sums and
 //                 the apply, so every tensor moves once.  Needs C a multiple of 4, groups of a power of two up to 256 channels or of any
-//                 number up to 64, and a slab of at most 256 KB (forward) / 128 KB per tensor (backward; with tanh 64 KB).
+//                 number up to 64, and a slab of at most 256 KB (forward) / 128 KB per tensor (backward).
 //   gn_partial + gn_apply   everything else: pixel chunks' sums to the workspace, then the apply pass reads x (and dy) again.
 // All arithmetic on elements is in 64 bits: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for memory
 // either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
@@ -19,10 +19,7 @@
 namespace mmdgan {
 
 constexpr int kGnMaxThreads = 512;                   // 256 VGPRs per wave: at most half of them hold the slab
-// float4 per thread and tensor; tanh's code costs registers that a backward with 16 does not have (its spills made 32x64x64x64
-// 78 us, in two passes it takes 48; and 64x8x8x512 23 us where half of the registers had to do, now 13)
-constexpr int kGnFwdRegs = 32;
-template <bool TANH> constexpr int kGnBwdRegs = TANH ? 8 : 16;
+constexpr int kGnFwdRegs = 32, kGnBwdRegs = 16;      // float4 per thread and tensor
 // ... and for slabs and groups that are no powers of two: half of it, 8 at most (ANY below)
 constexpr int gn_any_regs(int regs) { return regs / 2 < 8 ? regs / 2 : 8; }
 constexpr int kGnGrid = 1024;                        // workgroups of a launch: four per CU
@@ -50,7 +47,13 @@ template <bool TANH> __device__ __forceinline__ float gn_act(float z, float belo
     return z > 0.f ? z : below == 0.f ? 0.f : z * below;
 }
 template <bool TANH> __device__ __forceinline__ double gn_slope(double z, float below) {
-    if (TANH) { const double t = (double)tanhf((float)z); return 1.0 - t * t; }
+    if (TANH) {
+        // 1 - tanh^2 = 4 e / (1 + e)^2, e = exp(-2 |z|): one exponential and one reciprocal in 32 bits (both good to 2^-23).  In units of
+        // 2^-24: 1 + e, the reciprocal and the products 8; e itself 2 + 6 |z| (z's, the constant's and the product's rounding), of
+        // which tanh |z| counts: at most 9 of 1 in all, where 1 - t^2 from tanhf had 12.
+        const float e = __builtin_amdgcn_exp2f(-2.88539008f * fabsf((float)z)), r = __builtin_amdgcn_rcpf(1.f + e);
+        return (double)(4.f * e * r * r);
+    }
     return z > 0.0 ? 1.0 : (double)below;
 }
 // A value that the compiler must treat as new: without it the 64-bit conversions and normalised values of the first pass over
@@ -69,10 +72,13 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 // ANY: slabs and groups that are no powers of two - columns dealt to the threads by division, those that are left over idle, sums
 // through LDS from every thread instead of by shuffles.  64x8x8x320 in groups of 10: forward 7.8 us, backward 12.1 (in two passes 21.8 and
 // 30.9), 64x32x32x96 in groups of 3: 15.7 and 27.7 (16.7 and 31.6); with 16 float4 per thread and more the two passes win
-// (33x47x31x96: forward 14.0 us against 21.3), with tanh's code in the backward from 8 on (64x16x16x192: 20.0 against 26.9).
+// (33x47x31x96: forward 14.0 us against 21.3).
 // red: [row groups][NV][CV] doubles (ANY: [NV][T]), chan: [2][S] (backward totals of this workgroup), stat: [2][S].
+// Waves per SIMD that the registers are cut for: four where the slab's values leave room.  Four channels' own groups or tanh's slope
+// beside 4 float4 of x and dy spilled (64x16x16x64 in groups of two, backward: 12.0 us with the spills, 9.2 on half of the waves).
+constexpr int gn_waves(int U, bool bwd, bool tanh, int gp) { return (bwd ? U <= (tanh || gp == 4 ? 2 : 4) : U <= 8) ? 4 : 2; }
 template <int U, bool BWD, bool TANH, int GP, bool ANY>
-__global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8) ? 4 : 2) void gn_resident_kernel(GnArgs a) {
+__global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_resident_kernel(GnArgs a) {
     constexpr bool kByCol = !BWD && GP == 1;
     constexpr int NV = kByCol ? 2 : 8;
     extern __shared__ double gn_lds[];
@@ -138,13 +144,11 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
                     s[kByCol ? 0 : j] += v;
                     s[kByCol ? 1 : 4 + j] = fma(v, v, s[kByCol ? 1 : 4 + j]);
                 } else {                                   // (a pixel beyond the image holds dy = 0: it adds nothing)
-                    double dz = (double)dv[j] * gn_slope<TANH>(fma(A[j], v, B[j]), a.below);
-                    if (TANH) { dv[j] = (float)dz; dz = (double)dv[j]; }      // evaluated once: dz itself, in 32 bits, for the second pass
+                    const double dz = (double)dv[j] * gn_slope<TANH>(fma(A[j], v, B[j]), a.below);
                     s[j] += dz;
                     s[(4 + j) % NV] = fma(dz, v, s[(4 + j) % NV]);
                 }
             }
-            if (BWD && TANH) vd[u] = make_float4(dv[0], dv[1], dv[2], dv[3]);
         }
         // lanes of a wave that hold the same column
         if (!ANY) {
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(kGnMaxThreads, (BWD ? U <= (TANH ? 2 : 4) : U <= 8)
             for (int j = 0; j < 4; ++j) {
                 const double v = xv[j], z = fma(A[j], v, B[j]);
                 if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
-                else o[j] = (float)fma(A[j], TANH ? (double)dv[j] : (double)dv[j] * gn_slope<false>(z, a.below), fma(L[j % GP], v, M[j % GP]));
+                else o[j] = (float)fma(A[j], (double)dv[j] * gn_slope<TANH>(z, a.below), fma(L[j % GP], v, M[j % GP]));
             }
             if (r < HW) *reinterpret_cast<float4 *>(po + (size_t)r * a.C) = make_float4(o[0], o[1], o[2], o[3]);
         }
@@ -514,8 +518,8 @@ static void gn_plan_resident(long HW, int C, int D, long N, int regs, GnPlan &p)
     int top = 4;                                       // widest power-of-two slab that divides C
     while (top < kGnSplitCh && C % (top * 2) == 0) top *= 2;
     // ... of 4 or 8 channels reads 16 or 32 bytes of a pixel at a time: the other form's wider slabs first (64x16x16x200 in groups of one:
-    // forward 12.5 -> 10.2 us, backward 27.9 -> 19.2; with tanh's backward and 8 channels 20.8 -> 26.9, so not there)
-    if (!gn_pow2(D) || (top < (regs > 8 ? 16 : 8) && top < C)) {
+    // forward 12.5 -> 10.2 us, backward 27.9 -> 19.4)
+    if (!gn_pow2(D) || (top < 16 && top < C)) {
         gn_plan_any(HW, C, D, N, regs, p);
         if (p.resident || !gn_pow2(D)) return;
     }
@@ -569,7 +573,7 @@ static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st)
     const int CV = p.S / 4, wide = CV < 64 ? 64 : CV;
     const size_t lds = ((ANY ? (size_t)p.T * 8 : (size_t)(p.T / wide) * (!BWD && GP == 1 ? 2 : 8) * CV) + 4 * (size_t)p.S) * sizeof(double);
     const dim3 grid((unsigned)(a.rows * a.slabs)), block(p.T);
-    constexpr int REGS = BWD ? kGnBwdRegs<TANH> : kGnFwdRegs, MOST = ANY ? gn_any_regs(REGS) : REGS;      // U at most
+    constexpr int REGS = BWD ? kGnBwdRegs : kGnFwdRegs, MOST = ANY ? gn_any_regs(REGS) : REGS;      // U at most
     switch (p.U) {
         case 1: hipLaunchKernelGGL((gn_resident_kernel<1, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
         case 2: hipLaunchKernelGGL((gn_resident_kernel<2, BWD, TANH, GP, ANY>), grid, block, lds, st, a); break;
@@ -583,7 +587,7 @@ static void gn_launch_resident(const GnArgs &a, const GnPlan &p, hipStream_t st)
 template <bool BWD, bool TANH>
 static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipStream_t st, const char *what) {
     GnPlan p;
-    gn_plan_resident(a.HW, a.C, a.D, a.N, BWD ? kGnBwdRegs<TANH> : kGnFwdRegs, p);
+    gn_plan_resident(a.HW, a.C, a.D, a.N, BWD ? kGnBwdRegs : kGnFwdRegs, p);
     if (p.resident && !(gn_aligned(a.x) && gn_aligned(a.out) && gn_aligned(a.gamma) && gn_aligned(a.beta) && (!BWD || gn_aligned(a.dy))))
         p.resident = false;
     long part_rows;
