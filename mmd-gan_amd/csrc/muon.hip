@@ -21,9 +21,9 @@
 // 4 KB further apart than their blocks fill: with m a power of two all workgroups of a product, at the same reduction step, would
 // otherwise read addresses that are equal modulo 128 KB, from the same few memory channels.
 //
-// Measured (five steps; 21 launches): 4608x512 alone 146 us - thirteen m x m products of 5.5 us, latency, not work (24 us at the rate of
-// a large fp16 product); the 64x64 images' discriminator (24 M parameters) 0.96 ms: momentum and norm 92 us and the split 47 (HBM),
-// two Gram matrices 93 + 21 each (0.6 of a large product's rate), thirteen m x m products of 21, two products with X 167 and 186 (0.65).
+// Measured (five steps; 21 launches): 4608x512 alone 147 us - thirteen m x m products of 5.5 us, latency, not work (24 us at the rate of
+// a large fp16 product); the 64x64 images' discriminator (24 M parameters) 0.92 ms: momentum and norm 92 us and the split 47 (HBM),
+// two Gram matrices 92 + 21 each (0.6 of a large product's rate), thirteen m x m products of 21, two products with X 163 and 178 (0.67).
 #include "muon_internal.h"
 
 namespace mmdgan {
@@ -403,13 +403,13 @@ struct MuSquareTable { MuFirst<2 * kMuGroup> f; MuSquare j[2 * kMuGroup]; };
 
 // Latency-bound: no staging, tiles of 32 x 32 (136 workgroups from one matrix of m = 512), the four waves of a tile take the 32-wide
 // reduction steps in turn, each straight from L2 into MFMA operands with kMuAhead steps in flight, and their sums meet in LDS.
-// A launch at m = 512 takes 5.9 us (64 x 64 tiles on 36 workgroups: 9.8).  At m = 1024 the finer tiles read twice as much from L2 and
-// still win, several workgroups to a CU covering each other's waits: the whole update of the 64 x 64 images' discriminator takes 1.02 ms,
-// with 64 x 64 tiles above m = 512 it took 1.11.
+// A launch at m = 512 takes 5.5 us (64 x 64 tiles on 36 workgroups: 9.8).  At m = 1024 the finer tiles read twice as much from L2 and
+// still win, several workgroups to a CU covering each other's waits: 21 us for the products of the 64 x 64 images' discriminator, 270 MB
+// of operands at 12.5 TB/s.
 constexpr int kMuAhead = 2;
 
 // tile number -> (ti, tj), ti >= tj, of a triangle of nb rows: in blocks of 4 x 4 tiles where nb allows, so that an XCD's run of
-// neighbours needs few row blocks (that update without it: 1.04 ms)
+// neighbours needs few row blocks (that net's whole update without it 1.04 ms, with it 1.02, both at the time)
 __device__ __forceinline__ void mu_tri_blocked(int t, int nb, int &ti, int &tj) {
     if (nb & 3) { mu_tri(t, ti, tj); return; }
     int si = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.125f);        // 8 si^2 + 2 si tiles before block row si
