@@ -330,3 +330,37 @@ def test_what_a_matrix_gets_does_not_depend_on_the_others(ops, shapes):
         ops.MuonGroup([p], [u], [torch.zeros_like(u)]).step(0.1)
     ops.MuonGroup(ps, us, ms).step(0.1)
     assert all(torch.equal(p, q) for p, q in zip(ps, alone))
+
+
+def test_a_captured_update_advances_like_eager_ones(ops):
+    """momentum and parameters after replays of one captured update, eager work and synchronisations between them, are those of as many
+    eager updates, bit for bit; unaligned tensors and a second group on another stream beside it"""
+    shapes, g = [(27, 16), (300, 130), (64, 70), (129, 40), (70, 200)], torch.Generator().manual_seed(5)
+    host = [[torch.randn(*s, generator=g) * k for s in shapes] for k in (0.05, 1e-3, 1e-3)]
+
+    def odd(t):                                              # four bytes off a 16-byte boundary
+        f = torch.zeros(t.numel() + 1, device='cuda')
+        v = f[1:].view(t.shape)
+        v.copy_(t)
+        return v
+    eager, graphed, other = ([[f(t) for t in ts] for ts in host] for f in (lambda t: t.cuda(), lambda t: t.cuda(), odd))
+    groups = [ops.MuonGroup(*ts) for ts in (eager, graphed, other)]
+    groups[1].step(0.0, momentum=1.0, grad_scale=0.0)        # (allocates its workspace; moves nothing)
+    assert all(torch.equal(a, b) for a, b in zip(graphed[0] + graphed[2], eager[0] + eager[2]))
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        groups[1].step(0.02, momentum=0.9, weight_decay=0.01)
+    torch.cuda.synchronize()
+    for n in range(4):
+        groups[0].step(0.02, momentum=0.9, weight_decay=0.01)
+        if n % 2:
+            torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(s):
+            groups[2].step(0.02, momentum=0.9, weight_decay=0.01)
+        torch.cuda.synchronize()
+        for a, b, c in zip(eager[0] + eager[2], graphed[0] + graphed[2], other[0] + other[2]):
+            assert torch.equal(a, b), n
+            # (unaligned: the norm's sum in another order, its last bit in 64; that may flip roundings of X to 22 bits, 2^-22 of O's
+            # entries before products that keep them, times a step of at most 0.02 * 0.2 * sqrt(300) = 0.07: far below 2^-20 of 0.2)
+            assert float((a - c).abs().max()) <= 2.0 ** -20 * float(a.abs().max()), n
