@@ -5,6 +5,7 @@ hand-written HIP kernel through ctypes and fails loudly if the library or a gfx9
 missing.  Activations are NHWC fp32 tensors, kernels are in the reference's HWIO layout.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -487,7 +488,8 @@ def _on_current_device(*tensors):
     """launches go to the current device's current stream: a tensor that lives on another one is refused"""
     here = torch.cuda.current_device()
     for t in tensors:
-        assert t is None or t.get_device() == here, 'a tensor lives on device {}, the current one is {}'.format(t.get_device(), here)
+        if t is not None and t.get_device() != here:
+            raise AssertionError('a tensor lives on device {}, the current one is {}'.format(t.get_device(), here))
 
 
 def _gn_geometry(x, gamma, beta, groups):
@@ -495,10 +497,7 @@ def _gn_geometry(x, gamma, beta, groups):
     N, C = x.shape[0], x.shape[-1]
     assert max(N, C) < 1 << 31, 'group_norm: {} images of {} channels'.format(N, C)      # (they travel as C ints)
     assert gamma.numel() == C and beta.numel() == C, 'group_norm: gamma and beta have one entry per channel'
-    HW = 1
-    for s in x.shape[1:-1]:
-        HW *= s
-    return N, HW, C, int(groups)
+    return N, x.numel() // max(N * C, 1), C, int(groups)
 
 
 def _p64(t, shape):
@@ -507,8 +506,13 @@ def _p64(t, shape):
     return t.data_ptr()
 
 
+@functools.lru_cache(maxsize=1024)
+def _gn_bytes(N, HW, C, G):
+    return _lib.load().mmdgan_gn_workspace_bytes(N, HW, C, G)
+
+
 def _gn_ws(workspace, N, HW, C, G, device):
-    need = _lib.load().mmdgan_gn_workspace_bytes(N, HW, C, G)
+    need = _gn_bytes(N, HW, C, G)
     if workspace is None:
         return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
     assert workspace.is_cuda and workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need, \
