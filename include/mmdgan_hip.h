@@ -527,8 +527,8 @@ int mmdgan_adam_prepare_multi(const mmdgan_adam_prepare_job *jobs, int n, void *
  *                  rate serves a net whose vectors stay with Adam.  out may be param, momentum_out may be momentum.
  * Results are as near to the exact ones as 32-bit products on X give, for ill-conditioned and rank-deficient U too; sums in a fixed
  * order: equal inputs give equal bits (replicas of a data-parallel job stay identical).  All matrices of a call run
- * together, phase by phase, 16 at a time: 21 launches at five steps for those with both sides above 64, 3 for the others (in 64
- * bits: csrc/muon_small.hip).  jobs: HOST array, read during the call.  What a matrix writes may overlap nothing of the call but
+ * together, phase by phase, 16 at a time: 21 launches at five steps for those with both sides above 64, 3 per eight steps for the
+ * others (in 64 bits: csrc/muon_small.hip).  jobs: HOST array, read during the call.  What a matrix writes may overlap nothing of the call but
  * the input named above.
  * Shorter side <= 8192, longer <= 2^22, rows * cols < 2^31; 1 <= steps <= 16.
  * workspace: mmdgan_muon_workspace_bytes(jobs, n, steps) bytes (rows, cols of the jobs are read), 16-byte aligned, nothing kept in

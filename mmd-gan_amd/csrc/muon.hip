@@ -776,7 +776,7 @@ static size_t mu_bytes(const mmdgan_muon_job *jobs, int n, int steps, bool keep_
         size_t at = 0;
         for (int i = 0; i < k; ++i) {
             const mmdgan_muon_job &j = jobs[idx[i]];
-            at = small ? mu_round(at) + mu_small_bytes(j.rows, j.cols, keep_u) : mu_place(j.rows, j.cols, keep_u, steps, at).end;
+            at = small ? mu_round(at) + mu_small_bytes(j.rows, j.cols, keep_u, steps) : mu_place(j.rows, j.cols, keep_u, steps, at).end;
         }
         if (at > most) most = at;
     });

@@ -58,7 +58,7 @@ static inline size_t mu_round(size_t v) { return (v + 255) & ~(size_t)255; }
 // muon_small.hip: matrices whose shorter side is at most kMuSmall
 constexpr int kMuSmall = 64;
 static inline bool mu_is_small(int rows, int cols) { return (rows < cols ? rows : cols) <= kMuSmall; }
-size_t mu_small_bytes(int rows, int cols, bool keep_u);
+size_t mu_small_bytes(int rows, int cols, bool keep_u, int steps);
 void mu_small_run(const MuJob *jobs, int n, const MuStep &s, char *ws, hipStream_t st);
 
 }  // namespace mmdgan

@@ -1,14 +1,19 @@
-// Orthogonalised updates (muon.hip) of matrices whose shorter side m is at most 64: three launches, all products in 64 bits.
+// Orthogonalised updates (muon.hip) of matrices whose shorter side m is at most 64: three launches for up to eight steps, all
+// products in 64 bits.
 //
 //   gram     U = g (+ momentum) read, U kept, partial sums of A = U U^T over pieces of the longer side n
-//   chain    one workgroup per matrix: A / trace(A) (the trace is ||U||^2), every step of the polynomial on m x m matrices in LDS,
-//            P = Q_steps ... Q_1 / ||U||
+//   chain    one workgroup per matrix: A / trace(A) (the trace is ||U||^2), up to eight steps of the polynomial on m x m matrices in
+//            LDS, P = Q_steps ... Q_1 / ||U||
 //   apply    out = P U, or the parameter update with it
 //
-// With 64 bits no second Gram matrix is needed (muon.hip: rounding errors of A grow 12-fold per step) and U is never
-// normalised, so nothing is rounded before the result.  v_mfma_f64_16x16x4 runs at a quarter of the rate of the fp16 pairs of
-// muon.hip per product, but these products are small: what counts is launches (3 instead of 21) and their latency.  The chain is
-// one CU's work, 17 products of m^3 at 128 flop / cycle on one triangle's tiles with a barrier between each two: 34.7 us at m = 64,
+// U is never normalised, so nothing is rounded before P U.  What the chain does to A's rounding errors bounds its length: along a
+// direction that U hardly has, A's eigenvalue is noise, 2^-46 or so and of either sign, a step multiplies it by Q^2 <= 12, and once it
+// reaches -0.1 Q grows with it and the chain diverges (32x288 of rank one, one Gram matrix for all steps: singular values up to 13 after
+// 13 steps, 5e6 after 16).  Eight steps leave it at 12^8 2^-46 = 6e-6, which puts Q off by 1e-5 of itself along directions whose singular
+// value is still below 3e-3: less than rounding X = P U to 32 bits does.  So X is formed, and the next eight steps start from its own
+// Gram matrix.
+// v_mfma_f64_16x16x4 runs at a quarter of the rate of the fp16 pairs of muon.hip per product, but these products are small: what
+// counts is launches (3 instead of 21) and their latency.  The chain is one CU's work, 17 products of m^3 at 128 flop / cycle on one triangle's tiles with a barrier between each two: 34.7 us at m = 64,
 // 11.6 at m = 27; beyond 64 it would grow eightfold, and the four m x m buffers would not fit LDS.  A 27x64 kernel alone takes 20 us,
 // eight matrices of a width-8 net 54 (gram 9, chain 35, apply 10).
 #include "muon_internal.h"
@@ -19,6 +24,7 @@ typedef double d4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSmRows = 64;                  // rows of n per LDS tile
 constexpr int kSmPieces = 64;                // pieces of n at most: partial sums the chain adds up
+constexpr int kSmChain = 8;                  // steps from one Gram matrix
 constexpr int kSmGramStride = 80, kSmApplyStride = 68;   // floats: conflict-free for the operand reads of the two kernels
 
 struct SmMat {
@@ -27,7 +33,7 @@ struct SmMat {
     MuPtr<double> slab, p;                // [pieces][tiles][256]; [R][R]
     int m, n, mt, pieces, per;       // mt 16-wide tiles; per: rows of n in a piece (a multiple of kSmRows)
 };
-struct SmTable { MuFirst<kMuGroup> f; SmMat a[kMuGroup]; MuStep s; };
+struct SmTable { MuFirst<kMuGroup> f; SmMat a[kMuGroup]; MuStep s; int norm; };          // norm: the Gram matrix is U's, not an iterate's
 static_assert(sizeof(SmTable) <= 4096, "a launch's tables travel as kernel arguments");
 
 __device__ __forceinline__ d4 sm_mfma(double a, double b, d4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
@@ -148,7 +154,7 @@ template <int MT> __device__ __forceinline__ void sm_put(double *x, int ti, int 
 }
 
 template <int MT>
-__device__ void sm_chain(const SmMat &p, int steps, double *lds) {
+__device__ void sm_chain(const SmMat &p, int steps, bool norm, double *lds) {
     constexpr int R = 16 * MT, ST = R + 2, NT = MT * (MT + 1) / 2;
     double *A = lds, *Q = A + R * ST, *W = Q + R * ST, *P = W + R * ST;
     const int t = threadIdx.x, w = t >> 6, waves = 16;       // 1024 threads
@@ -184,8 +190,8 @@ __device__ void sm_chain(const SmMat &p, int steps, double *lds) {
     __syncthreads();
     double tr = (t & 63) < R ? A[(t & 63) * (ST + 1)] : 0.0;
     tr = wave_sum(tr);                                       // ||U||^2, the same in every wave
-    const double inv = tr > 0.0 ? 1.0 / tr : tr == 0.0 ? 0.0 : tr;
-    const double psc = tr > 0.0 ? 1.0 / sqrt(tr) : tr == 0.0 ? 0.0 : tr;                     // (NaN stays NaN)
+    const double inv = !norm ? 1.0 : tr > 0.0 ? 1.0 / tr : tr == 0.0 ? 0.0 : tr;
+    const double psc = !norm ? 1.0 : tr > 0.0 ? 1.0 / sqrt(tr) : tr == 0.0 ? 0.0 : tr;       // (NaN stays NaN)
     __syncthreads();
     for (int e = t; e < R * R; e += blockDim.x) A[e / R * ST + e % R] *= inv;
     __syncthreads();
@@ -244,9 +250,9 @@ __device__ void sm_chain(const SmMat &p, int steps, double *lds) {
 __global__ __launch_bounds__(1024) void mu_small_chain_kernel(SmTable t) {
     extern __shared__ double sm_lds[];
     const SmMat &p = t.a[blockIdx.x];
-    if (p.mt == 1) sm_chain<1>(p, t.s.steps, sm_lds);
-    else if (p.mt == 2) sm_chain<2>(p, t.s.steps, sm_lds);
-    else sm_chain<4>(p, t.s.steps, sm_lds);
+    if (p.mt == 1) sm_chain<1>(p, t.s.steps, t.norm, sm_lds);
+    else if (p.mt == 2) sm_chain<2>(p, t.s.steps, t.norm, sm_lds);
+    else sm_chain<4>(p, t.s.steps, t.norm, sm_lds);
 }
 
 template <int MT>
@@ -321,7 +327,8 @@ __global__ __launch_bounds__(256) void mu_small_apply_kernel(SmTable t) {
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 struct SmPlace { int m, n, mt, pieces, per; size_t slab, p, u, end; };
-static SmPlace sm_place(int rows, int cols, bool keep_u, size_t base) {
+// scratch: U where it is kept, and X between two chains in the same place
+static SmPlace sm_place(int rows, int cols, bool scratch, size_t base) {
     SmPlace s{};
     s.m = rows < cols ? rows : cols; s.n = rows < cols ? cols : rows;
     s.mt = s.m <= 16 ? 1 : s.m <= 32 ? 2 : 4;
@@ -332,39 +339,58 @@ static SmPlace sm_place(int rows, int cols, bool keep_u, size_t base) {
     auto take = [&](size_t bytes) { const size_t at = o; o += mu_round(bytes); return at; };
     s.slab = take((size_t)s.pieces * (s.mt * (s.mt + 1) / 2) * 256 * sizeof(double));
     s.p = take((size_t)s.mt * s.mt * 256 * sizeof(double));
-    s.u = keep_u ? take((size_t)rows * cols * 4) : 0;
+    s.u = scratch ? take((size_t)rows * cols * 4) : 0;
     s.end = o;
     return s;
 }
-size_t mu_small_bytes(int rows, int cols, bool keep_u) { return sm_place(rows, cols, keep_u, 0).end; }
+size_t mu_small_bytes(int rows, int cols, bool keep_u, int steps) { return sm_place(rows, cols, keep_u || steps > kSmChain, 0).end; }
 
 void mu_small_run(const MuJob *jobs, int n, const MuStep &s, char *ws, hipStream_t st) {
     SmTable t{};
     t.s = s;
+    t.norm = 1;
     size_t at = 0;
-    unsigned gram = 0, apply = 0, first_apply[kMuGroup] = {};
+    unsigned gram = 0, apply = 0, first_gram[kMuGroup] = {}, first_apply[kMuGroup] = {};
+    float *x[kMuGroup];                                      // an iterate between two chains: in U's place, or where U would be
     int widest = 1;
     for (int i = 0; i < n; ++i) {
         const bool keep_u = jobs[i].mom.p && s.nesterov;
-        const SmPlace pl = sm_place(jobs[i].rows, jobs[i].cols, keep_u, at);
+        const SmPlace pl = sm_place(jobs[i].rows, jobs[i].cols, keep_u || s.steps > kSmChain, at);
         at = pl.end;
         SmMat &p = t.a[i];
         p.j = jobs[i];
-        p.u = keep_u ? (float *)(ws + pl.u) : nullptr;
+        x[i] = (float *)(ws + pl.u);
+        p.u = keep_u ? x[i] : nullptr;
         p.slab = (double *)(ws + pl.slab); p.p = (double *)(ws + pl.p);
         p.m = pl.m; p.n = pl.n; p.mt = pl.mt; p.pieces = pl.pieces; p.per = pl.per;
-        t.f.first[i] = gram; first_apply[i] = apply;
+        first_gram[i] = gram; first_apply[i] = apply;
         gram += pl.pieces; apply += (pl.n + kSmRows - 1) / kSmRows;
         if (pl.mt > widest) widest = pl.mt;
     }
     mu_close(t.f, n);
-    hipLaunchKernelGGL(mu_small_gram_kernel, dim3(gram), dim3(256), 0, st, t);
     const size_t lds = (size_t)4 * 16 * widest * (16 * widest + 2) * sizeof(double);         // up to 132 KB
     static const hipError_t allowed = hipFuncSetAttribute((const void *)mu_small_chain_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                           4 * 64 * 66 * (int)sizeof(double));
     (void)allowed;                                           // (a launch that it would have allowed reports the failure)
-    hipLaunchKernelGGL(mu_small_chain_kernel, dim3(n), dim3(1024), lds, st, t);
-    for (int i = 0; i < n; ++i) t.f.first[i] = first_apply[i];
-    hipLaunchKernelGGL(mu_small_apply_kernel, dim3(apply), dim3(256), 0, st, t);
+    for (int done = 0; done < s.steps; done += t.s.steps) {
+        t.s.steps = s.steps - done < kSmChain ? s.steps - done : kSmChain;
+        const bool last = done + t.s.steps == s.steps;
+        for (int i = 0; i < n; ++i) t.f.first[i] = first_gram[i];
+        hipLaunchKernelGGL(mu_small_gram_kernel, dim3(gram), dim3(256), 0, st, t);
+        hipLaunchKernelGGL(mu_small_chain_kernel, dim3(n), dim3(1024), lds, st, t);
+        for (int i = 0; i < n; ++i) {
+            t.f.first[i] = first_apply[i];
+            if (last) { t.a[i].j.out = jobs[i].out; t.a[i].j.param = jobs[i].param; }
+            else { t.a[i].j.out = x[i]; t.a[i].j.param = nullptr; }
+        }
+        hipLaunchKernelGGL(mu_small_apply_kernel, dim3(apply), dim3(256), 0, st, t);
+        // the next chain's U is X as it stands
+        t.norm = 0;
+        t.s.grad_scale = 1.f;
+        for (int i = 0; i < n; ++i) {
+            t.a[i].u = nullptr;
+            t.a[i].j.grad = x[i]; t.a[i].j.mom = nullptr; t.a[i].j.dsigma = nullptr;
+        }
+    }
 }
 }  // namespace mmdgan
