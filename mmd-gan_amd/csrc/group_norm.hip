@@ -566,6 +566,9 @@ static size_t gn_bytes(long N, long HW, int C, int G) {
     return gpart + part + 256;
 }
 
+// the sizes that the entries take: an image's offsets fit an int, a batch a grid dimension
+static bool gn_sizes_ok(int N, long HW, int C, int G) { return N >= 1 && HW >= 1 && C >= 1 && G >= 1 && C % G == 0 && N <= 65535 && HW <= 0x7fffffffL / C; }
+
 static bool gn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 template <bool BWD, bool TANH, int GP, bool ANY>
@@ -632,13 +635,12 @@ using namespace mmdgan;
 #define GN_REQUIRE_GEOMETRY(what)                                                                                                    \
     MMDGAN_REQUIRE(N >= 1 && HW >= 1 && C >= 1 && G >= 1, what ": bad size N=%d HW=%ld C=%d G=%d", N, HW, C, G);                      \
     MMDGAN_REQUIRE(C % G == 0, what ": %d channels do not divide into %d groups", C, G);                                              \
-    MMDGAN_REQUIRE(N <= 65535 && HW <= 0x7fffffffL / C, what ": image of %ld pixels x %d channels or batch of %d is too large", HW, C, N); \
+    MMDGAN_REQUIRE(gn_sizes_ok(N, HW, C, G), what ": image of %ld pixels x %d channels or batch of %d is too large", HW, C, N); \
     MMDGAN_REQUIRE(!((uintptr_t)workspace & 15), what ": the workspace is not 16-byte aligned");                                       \
     MMDGAN_REQUIRE(act >= MMDGAN_ACT_LINEAR && act <= MMDGAN_ACT_TANH, what ": unknown activation %d", act)
 
 extern "C" size_t mmdgan_gn_workspace_bytes(int N, long HW, int C, int G) {
-    if (N < 1 || HW < 1 || C < 1 || G < 1 || C % G) return 0;
-    return gn_bytes(N, HW, C, G);
+    return gn_sizes_ok(N, HW, C, G) ? gn_bytes(N, HW, C, G) : 0;
 }
 extern "C" int mmdgan_gn_fwd(const float *x, int N, long HW, int C, int G, const float *gamma, const float *beta, float eps, int act,
                              float *y, double *stats, void *workspace, void *stream) {

@@ -816,7 +816,7 @@ class TapeEngine:
 
     def _gn_scratch(self, key, n, x_shape, groups):
         hw = int(np.prod(x_shape[1:-1]))
-        return self._raw(key, int(ops.require_device().mmdgan_gn_workspace_bytes(n, hw, x_shape[-1], groups)))
+        return self._raw(key, max(int(ops.require_device().mmdgan_gn_workspace_bytes(n, hw, x_shape[-1], groups)), 16))     # (0: the entry refuses)
 
     def _sn_chain_layer(self, net, k):
         """the power iteration of kernel `k` as ops.SnChains describes it (the tensors of _sn_step), or None for a kernel with a

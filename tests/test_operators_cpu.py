@@ -148,3 +148,18 @@ def test_sides_that_do_not_fit_an_int_are_refused():
     g = torch.empty(1, device='meta').expand((1 << 32) + 4)
     with pytest.raises(AssertionError, match='4294967300'):
         ops._gn_geometry(g[None], g, g, 4)
+
+
+def test_group_norm_has_no_workspace_for_sizes_the_entries_refuse(lib):
+    """0 bytes, as documented, for every size that the entries refuse - also for one whose chunk length does not fit an int (it divided by
+    zero once)"""
+    size = lib.mmdgan_gn_workspace_bytes
+    for N, HW, C, G in ((65536, 9, 12, 3), (70000, 9, 12, 3), (2, 1 << 30, 12, 3), (1, 1 << 38, 4, 1), (1, 1 << 38, 1, 1), (1, (1 << 63) - 1, 1, 1),
+                        (1, -5, 4, 1), (2, 0, 4, 1), (2, 9, 0, 1), (2, 9, 12, 0), (2, 9, 12, -3)):
+        assert size(N, HW, C, G) == 0, (N, HW, C, G)
+        assert lib.mmdgan_gn_fwd(16, N, HW, C, G, 16, 16, 1e-5, 0, 16, 16, 16, None) == -1
+    assert size(65535, 9, 12, 3) > 0 and size(1, 0x7fffffff, 1, 1) > 0 and size(1, 0x7fffffff // 12, 12, 3) > 0
+    from mmdgan_hip import ops
+    for N, HW, C, G in ((65536, 9, 12, 3), (1, 1 << 38, 4, 1)):
+        with pytest.raises(ValueError, match='group_norm'):
+            ops.group_norm_workspace(N, HW, C, G, 'cpu')
