@@ -301,8 +301,8 @@ __global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
     const int chunk = blockIdx.y, n = blockIdx.z, ns = gn_src(a, n);
     const GnSlab sl = gn_slab(a, blockIdx.x);
     const int CV = (sl.width + VEC - 1) / VEC, RT = 256 / CV, rl = t / CV, col = t % CV;
-    const int p0 = chunk * a.chunk_px;
-    const int p1 = p0 + a.chunk_px < a.HW ? p0 + a.chunk_px : a.HW;
+    const int p0 = chunk * a.chunk_px;                 // rows are counted from the chunk's first: p0 + chunk_px may pass an int
+    const int rows = a.HW - p0 < a.chunk_px ? a.HW - p0 : a.chunk_px;
     double s1[VEC], s2[VEC], mean[VEC], rstd[VEC], ga[VEC], be[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { s1[j] = 0.0; s2[j] = 0.0; }
@@ -315,14 +315,14 @@ __global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
                 mean[j] = st[0]; rstd[j] = st[1]; ga[j] = a.gamma[c + j]; be[j] = a.beta[c + j];
             }
         }
-        const float *px = a.x + (size_t)ns * a.HW * a.C + c;
-        const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
-        for (int r = p0 + rl; r < p1; r += RT * U) {
+        const float *px = a.x + ((size_t)ns * a.HW + p0) * a.C + c;
+        const float *pd = BWD ? a.dy + ((size_t)n * a.HW + p0) * a.C + c : nullptr;
+        for (int r = rl; r < rows; r += RT * U) {
             float vx[U][VEC], vd[U][VEC];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int rr = r + u * RT;
-                const bool ok = rr < p1;
+                const bool ok = rr < rows;
                 if (ok) gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
                 if (BWD && ok) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
                 if (!ok) {
@@ -386,8 +386,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
     const int chunk = blockIdx.y, n = blockIdx.z, ns = gn_src(a, n);
     const GnSlab sl = gn_slab(a, blockIdx.x);
     const int CV = (sl.width + VEC - 1) / VEC, RT = 256 / CV, rl = t / CV, col = t % CV;
-    const int p0 = chunk * a.chunk_px;
-    const int p1 = p0 + a.chunk_px < a.HW ? p0 + a.chunk_px : a.HW;
+    const int p0 = chunk * a.chunk_px;                 // rows are counted from the chunk's first: p0 + chunk_px may pass an int
+    const int rows = a.HW - p0 < a.chunk_px ? a.HW - p0 : a.chunk_px;
     const int P = a.chunks * a.pieces;
     const double inv_m = 1.0 / ((double)a.HW * a.D);
     auto publish = [&](int g, double u1, double u2) {
@@ -403,18 +403,18 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
         }
     };
     const int c = sl.c0 + col * VEC;
-    const float *px = a.x + (size_t)ns * a.HW * a.C + c;
-    const float *pd = BWD ? a.dy + (size_t)n * a.HW * a.C + c : nullptr;
+    const float *px = a.x + ((size_t)ns * a.HW + p0) * a.C + c;
+    const float *pd = BWD ? a.dy + ((size_t)n * a.HW + p0) * a.C + c : nullptr;
     float vx[U][VEC], vd[BWD ? U : 1][VEC];
     auto fetch = [&](int r) {                          // (a row beyond the chunk: its last row again, never used)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int rr = r + u * RT < p1 ? r + u * RT : p1 - 1;
+            const int rr = r + u * RT < rows ? r + u * RT : rows - 1;
             gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
             if (BWD) gn_load<VEC>(pd + (size_t)rr * a.C, vd[BWD ? u : 0]);
         }
     };
-    fetch(p0 + rl);                                    // in flight while the statistics come together
+    fetch(rl);                                         // in flight while the statistics come together
     const int lanes = gn_lanes(sl.groups), mine = t / lanes, l = t & (lanes - 1);
     double u1 = 0.0, u2 = 0.0;
     if (mine < sl.groups) {
@@ -442,9 +442,9 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
         A[j] = rstd * (double)a.gamma[c + j];
         B[j] = fma(-mean, A[j], (double)a.beta[c + j]);
     }
-    float *po = a.out + (size_t)n * a.HW * a.C + c;
-    for (int r = p0 + rl; r < p1; r += RT * U) {
-        if (r != p0 + rl) fetch(r);
+    float *po = a.out + ((size_t)n * a.HW + p0) * a.C + c;
+    for (int r = rl; r < rows; r += RT * U) {
+        if (r != rl) fetch(r);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int rr = r + u * RT;
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
                 if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
                 else o[j] = (float)fma(A[j], (double)vd[BWD ? u : 0][j] * gn_slope<TANH>(z, a.below), fma(L[j], v, M[j]));
             }
-            if (rr < p1) {
+            if (rr < rows) {
                 if (VEC == 4) *reinterpret_cast<float4 *>(po + (size_t)rr * a.C) = make_float4(o[0], o[1 % VEC], o[2 % VEC], o[3 % VEC]);
                 else po[(size_t)rr * a.C] = o[0];
             }
@@ -544,7 +544,7 @@ static void gn_plan_resident(long HW, int C, int D, long N, int regs, GnPlan &p)
 }
 static void gn_plan_split(long HW, int C, int D, long N, GnPlan &p) {
     const int G = C / D;
-    if (D <= kGnSplitCh) { p.gps = kGnSplitCh / D < G ? kGnSplitCh / D : G; p.pieces = 1; p.SB = p.gps * D; p.slabs = (G + p.gps - 1) / p.gps; }
+    if (D <= kGnSplitCh) { p.gps = kGnSplitCh / D < G ? kGnSplitCh / D : G; p.pieces = 1; p.SB = p.gps * D; p.slabs = (G - 1) / p.gps + 1; }
     else { p.gps = 1; p.pieces = (D + kGnSplitCh - 1) / kGnSplitCh; p.SB = kGnSplitCh; p.slabs = G * p.pieces; }
     // pixel chunks: four workgroups per CU in all, at least 64 pixels each
     long want = (4L * 256 + N * p.slabs - 1) / (N * p.slabs), most = (HW + 63) / 64;
@@ -619,7 +619,7 @@ static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipSt
             hipLaunchKernelGGL((gn_apply_kernel<1, BWD, TANH>), grid, block, 0, st, a);
         }
     }
-    if (params) hipLaunchKernelGGL(gn_param_kernel, dim3((a.C + 7) / 8), dim3(256), 0, st, a.part, part_rows, a.C, dgamma, dbeta);
+    if (params) hipLaunchKernelGGL(gn_param_kernel, dim3((a.C - 1) / 8 + 1), dim3(256), 0, st, a.part, part_rows, a.C, dgamma, dbeta);
     return check_launch(what);
 }
 template <bool BWD>
