@@ -11,9 +11,11 @@
 //                 the apply, so every tensor moves once.  Needs C a multiple of 4, groups of a power of two up to 256 channels or of any
 //                 number up to 64, and a slab of at most 256 KB (forward) / 128 KB per tensor (backward).
 //   gn_partial + gn_apply   everything else: pixel chunks' sums to the workspace, then the apply pass reads x (and dy) again.
-// All arithmetic on elements is in 64 bits: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for memory
-// either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
-// cancel cleanly from dx.  The sums are formed in a fixed order, without atomics: equal inputs give equal bits.
+// Arithmetic on elements is in 64 bits, but for tanh and its slope: v_fma_f64 issues at the fp32 rate on this part, the kernels wait for
+// memory either way, and with it the sign that relu / lrelu take is the one the exact value has and a group's own mean and variance
+// cancel cleanly from dx, wherever the mean lies (kGnFar below).  The sums are formed in a fixed order, without atomics: equal inputs
+// give equal bits.
+#include <type_traits>
 #include "common.h"
 
 namespace mmdgan {
@@ -30,7 +32,7 @@ struct GnArgs {
     double *stats;               // [N][G][2]: mean, rstd
     float *out;                  // y / dx
     double *part;                // backward: [rows][2][C] partial dbeta, dgamma (null: not wanted)
-    double *gpart;               // two-pass form: [N][G][P][2]
+    double *gpart, *pivot;       // two-pass form: [N][G][P][2]; forward: [N][G]
     int N, x_batch, HW, C, G, D;
     float below;                 // the activation's slope below zero
     float eps;
@@ -59,6 +61,20 @@ template <bool TANH> __device__ __forceinline__ double gn_slope(double z, float 
 // A value that the compiler must treat as new: without it the 64-bit conversions and normalised values of the first pass over
 // a thread's elements are kept across the barrier for the second (U * 16 more registers: spills from U = 8 on).
 __device__ __forceinline__ void gn_fresh(float4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+// Means far from zero.  E[x^2] - mean^2 in 64 bits loses (mean rstd)^2 2^-53 of the variance, nothing that counts while the mean is a
+// few standard deviations, but 1e-4 at 10^6 of them and all of it for a constant group; and A x + B, below, is off by |mean| rstd 2^-53.
+// - Statistics: around the group's first value k, whatever part of the group a workgroup sums, E[(x - k)^2] - E[x - k]^2 loses M 2^-53 at
+//   most, k lying within sqrt(M) standard deviations of the mean.  The two-pass form always subtracts k; in the resident form that
+//   subtraction shows (256x64x64x64 in groups of 4: 138 -> 142 us): it sums x itself and reads a slab once more, from L2, where a mean
+//   turns out to be far (64x32x32x64 at a mean of 10^5 deviations: in groups of 8 10.0 -> 12.6 us, in groups of 2 11.6 -> 20.1).
+// - Maps and the backward sums take x - c, c = the mean rounded to 32 bits where it is far, else 0.  The 32-bit difference is exact for
+//   x within a factor of two of c; a value further out is sqrt(M) standard deviations away at most, and off by 2^-24 of that.
+constexpr double kGnFar = 256.0;
+__device__ __forceinline__ bool gn_far(double mean, double rstd) { return fabs(mean) * rstd > kGnFar; }
+__device__ __forceinline__ float gn_centre(double mean, double rstd) { return gn_far(mean, rstd) ? (float)mean : 0.f; }
+// (k: 0 if the first value is infinite or NaN, which then reaches mean and variance through the sums)
+__device__ __forceinline__ float gn_finite(float k) { return fabsf(k) < __builtin_inff() ? k : 0.f; }
+__device__ __forceinline__ void gn_subtract(float4 &v, float x, float y, float z, float w) { v.x -= x; v.y -= y; v.z -= z; v.w -= w; }
 // image of x (and of stats) that output image n reads: the images beyond x_batch take the last ones again
 __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_batch ? n : n - (a.N - a.x_batch); }
 
@@ -70,17 +86,24 @@ __device__ __forceinline__ int gn_src(const GnArgs &a, int n) { return n < a.x_b
 // GP: groups that a thread's four channels can belong to - 1 if D is a multiple of 4 (fewer registers, and the forward sums of the
 // four are one), else 4.  An item of the reduction is a channel, or (forward, GP = 1) a column of four.
 // ANY: slabs and groups that are no powers of two - columns dealt to the threads by division, those that are left over idle, sums
-// through LDS from every thread instead of by shuffles.  64x8x8x320 in groups of 10: forward 7.8 us, backward 12.1 (in two passes 21.8 and
-// 30.9), 64x32x32x96 in groups of 3: 15.7 and 27.7 (16.7 and 31.6); with 16 float4 per thread and more the two passes win
-// (33x47x31x96: forward 14.0 us against 21.3).
-// red: [row groups][NV][CV] doubles (ANY: [NV][T]), chan: [2][S] (backward totals of this workgroup), stat: [2][S].
+// through LDS from every thread instead of by shuffles.  64x8x8x320 in groups of 10: forward 6.3 us, backward 10.3 (in two passes 15.9 and
+// 28.6), 64x32x32x96 in groups of 3: 15.6 and 27.7 (16.5 and 30.7); with 16 float4 per thread and more the two passes win
+// (33x47x31x96: forward 14.5 us against 21.3).
+// Forward, one thread of a group forms its mean and rstd, the others read them: the square roots and divisions of a thread's four
+// groups, side by side, cost the registers that hold the slab (64x32x32x64 in groups of 2: 12.4 us, now 11.6).
+// red: [row groups][NV][CV] doubles (ANY: [NV][T]), chan: [2][S] (backward: totals of this workgroup), stat: [2][S] (forward:
+// mean and rstd, by group).
 // Waves per SIMD that the registers are cut for: four where the slab's values leave room.  Four channels' own groups or tanh's slope
 // beside 4 float4 of x and dy spilled (64x16x16x64 in groups of two, backward: 12.0 us with the spills, 9.2 on half of the waves).
+// Forward with 8 float4 and four channels' own groups 14 to 20 registers spill; on half of the waves none do, and 256x16x16x96 in groups
+// of 3 takes 15.9 us instead of 13.3 (64x32x32x64 in groups of 2: 11.6 either way).  A few more spill where the slab takes half of 256
+// registers (32 float4 forward, 16 backward) and backward with 2 float4 and four channels' own groups.
 constexpr int gn_waves(int U, bool bwd, bool tanh, int gp) { return (bwd ? U <= (tanh || gp == 4 ? 2 : 4) : U <= 8) ? 4 : 2; }
 template <int U, bool BWD, bool TANH, int GP, bool ANY>
 __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_resident_kernel(GnArgs a) {
     constexpr bool kByCol = !BWD && GP == 1;
     constexpr int NV = kByCol ? 2 : 8;
+    constexpr bool kOnce = BWD && GP == 4;             // x - c kept from the sums: four c held through the barrier are too many
     extern __shared__ double gn_lds[];
     const int T = blockDim.x, t = threadIdx.x, lane = t & 63;
     const int S = a.S, CV = S >> 2, RT = T / CV, D = a.D, HW = a.HW;
@@ -89,6 +112,7 @@ __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_
     double *red = gn_lds;
     double *chan = red + (ANY ? T * NV : RG * NV * CV);
     double *stat = chan + 2 * S;
+    int *again = reinterpret_cast<int *>(chan);        // forward: whether the slab's sums are taken around its groups' first values
     // the slabs of an image share its cache lines: neighbours on one XCD (workgroups go to the eight XCDs in turn, each has its own
     // L2) and close in time - of every 8 images, slab fastest, an XCD takes an eighth
     const int group = blockIdx.x / (8 * a.slabs), in = blockIdx.x - group * 8 * a.slabs;
@@ -98,8 +122,8 @@ __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_
     const int c0 = slab * S + col * 4, g0 = slab * S / D;
     const int items = kByCol ? CV : S, per_group = kByCol ? D >> 2 : D;      // items, and items per group
     const int DW = ANY ? 1 : per_group < 64 ? per_group : 64;        // neighbours that one wave reduces by shuffles
-    int LN = 64;                                       // ANY: lanes that share an item
-    while (LN > 1 && S * LN > T) LN >>= 1;
+    int LN = 64;                                       // ANY: lanes that share a channel (backward) or a group
+    while (LN > 1 && (BWD ? S : S / D) * LN > T) LN >>= 1;
     const int per = per_group / DW;
     const float4 gv = *reinterpret_cast<const float4 *>(a.gamma + c0), bv = *reinterpret_cast<const float4 *>(a.beta + c0);
     const float ga[4] = {gv.x, gv.y, gv.z, gv.w}, be[4] = {bv.x, bv.y, bv.z, bv.w};
@@ -119,22 +143,28 @@ __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_
             vx[u] = ok ? *reinterpret_cast<const float4 *>(px + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
             if (BWD) vd[u] = ok ? *reinterpret_cast<const float4 *>(pd + (size_t)r * a.C) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        double A[4], B[4], mean[GP], rstd[GP];
+        double A[4], B[4], mean[GP], rstd[GP];             // mean: of x - cf
+        float cf[GP];
         if (BWD) {
 #pragma unroll
             for (int j = 0; j < GP; ++j) {
                 const double *st = a.stats + 2 * ((size_t)ns * a.G + (c0 + j) / D);
-                mean[j] = st[0]; rstd[j] = st[1];
+                rstd[j] = st[1];
+                cf[j] = gn_centre(st[0], rstd[j]);
+                mean[j] = st[0] - (double)cf[j];
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) { A[j] = rstd[j % GP] * (double)ga[j]; B[j] = fma(-mean[j % GP], A[j], (double)be[j]); }
         }
-        double s[NV];
+        double s[NV], L[GP], M[GP];
 #pragma unroll
         for (int k = 0; k < NV; ++k) s[k] = 0.0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+            float4 w = vx[u];
+            if (BWD) gn_subtract(w, cf[0], cf[1 % GP], cf[2 % GP], cf[3 % GP]);
+            if (kOnce) vx[u] = w;
+            const float xv[4] = {w.x, w.y, w.z, w.w};
             float dv[4] = {0.f, 0.f, 0.f, 0.f};
             if (BWD) { dv[0] = vd[u].x; dv[1] = vd[u].y; dv[2] = vd[u].z; dv[3] = vd[u].w; }
 #pragma unroll
@@ -150,85 +180,133 @@ __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_
                 }
             }
         }
-        // lanes of a wave that hold the same column
-        if (!ANY) {
-            for (int o = 32; o >= CV; o >>= 1) {
+        auto gather = [&](auto first) {                    // s to the groups' totals (forward: mean, rstd) in stat, through two barriers
+            constexpr bool FIRST = decltype(first)::value;
+            // lanes of a wave that hold the same column
+            if (!ANY) {
+                for (int o = 32; o >= CV; o >>= 1) {
 #pragma unroll
-                for (int k = 0; k < NV; ++k) s[k] += __shfl_xor(s[k], o, 64);
-            }
-        }
-        if (ANY) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k) red[k * T + t] = s[k];
-        } else if (CV >= 64 || lane < CV) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k) red[(rg * NV + k) * CV + col] = s[k];
-        }
-        __syncthreads();
-        // totals over the row groups, then over the group's items
-        for (int i0 = 0; i0 < (ANY ? S : items); i0 += ANY ? T / LN : T) {
-            const int i = i0 + (ANY ? t / LN : t);
-            if (!ANY && i >= items) break;
-            const int k = kByCol ? 0 : i & 3, q = kByCol ? i : i >> 2;
-            double s1 = 0.0, s2 = 0.0;
-            if (ANY) {
-                if (i < S)
-                    for (int z = t & (LN - 1); z < RT; z += LN) {
-                        s1 += red[k * T + z * CV + q];
-                        s2 += red[(4 + k) * T + z * CV + q];
-                    }
-                for (int o = LN >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
-                if (i >= S || (t & (LN - 1))) continue;
-            } else {
-                for (int z = 0; z < RG; ++z) {
-                    s1 += red[(z * NV + k) * CV + q];
-                    s2 += red[(z * NV + (kByCol ? 1 : 4) + k) * CV + q];
+                    for (int k = 0; k < NV; ++k) s[k] += __shfl_xor(s[k], o, 64);
                 }
             }
-            if (BWD) {
-                const double *st = a.stats + 2 * ((size_t)ns * a.G + (slab * S + i) / D);
-                s2 = st[1] * fma(-st[0], s1, s2);
-                if (a.part && n < a.x_batch) { chan[i] += s1; chan[S + i] += s2; }
-                const double g = (double)a.gamma[slab * S + i];
-                s1 *= g; s2 *= g;
-            }
-            for (int o = DW >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
-            if ((i & (DW - 1)) == 0) { stat[i / DW] = s1; stat[S + i / DW] = s2; }
-        }
-        __syncthreads();
-        double L[GP], M[GP];
+            if (ANY) {
 #pragma unroll
-        for (int j = 0; j < GP; ++j) {
-            const int g = (col * 4 + j) / D;
-            if (ANY && j && g == (col * 4 + j - 1) / D) {    // (the same group as the channel before)
-                mean[j] = mean[j ? j - 1 : 0]; rstd[j] = rstd[j ? j - 1 : 0];
-                if (BWD) { L[j] = L[j ? j - 1 : 0]; M[j] = M[j ? j - 1 : 0]; }
-                continue;
+                for (int k = 0; k < NV; ++k) red[k * T + t] = s[k];
+            } else if (CV >= 64 || lane < CV) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) red[(rg * NV + k) * CV + col] = s[k];
             }
-            double s1 = 0.0, s2 = 0.0;
-            for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
-            s1 *= inv_m; s2 *= inv_m;
-            if (BWD) {
-                L[j] = -rstd[j] * rstd[j] * s2;
-                M[j] = -fma(L[j], mean[j], rstd[j] * s1);
-            } else {
-                double var = fma(-s1, s1, s2);
+            if (!BWD && FIRST && t == 0) *again = 0;
+            __syncthreads();
+            // group g of the slab, by one thread
+            auto publish = [&](int g, double s1, double s2) {
+                const double k = FIRST ? 0.0 : (double)gn_finite(px[g * D - col * 4]), m1 = s1 * inv_m, m2 = s2 * inv_m;
+                double var = fma(-m1, m1, m2);
                 if (var < 0.0) var = 0.0;
-                mean[j] = s1; rstd[j] = 1.0 / sqrt(var + (double)a.eps);
+                const double rstd = 1.0 / sqrt(var + (double)a.eps);
+                if (FIRST && gn_far(m1, rstd)) *again = 1;
+                double *st = a.stats + 2 * ((size_t)n * a.G + g0 + g);
+                st[0] = stat[g] = k + m1;
+                st[1] = stat[S + g] = rstd;
+            };
+            if (ANY && !BWD) {                             // LN lanes share a group's RT x W values
+                const int W = kByCol ? D >> 2 : D, second = kByCol ? T : 4 * T, step_r = LN / W, step_c = LN % W;
+                for (int i0 = 0; i0 < S / D; i0 += T / LN) {
+                    const int g = i0 + t / LN;
+                    double s1 = 0.0, s2 = 0.0;
+                    if (g < S / D)
+                        for (int z = (t & (LN - 1)) / W, d = (t & (LN - 1)) % W; z < RT;) {
+                            const int c = g * W + d, at = kByCol ? z * CV + c : (c & 3) * T + z * CV + (c >> 2);
+                            s1 += red[at];
+                            s2 += red[second + at];
+                            z += step_r; d += step_c;
+                            if (d >= W) { d -= W; ++z; }
+                        }
+                    for (int o = LN >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+                    if (g < S / D && !(t & (LN - 1))) publish(g, s1, s2);
+                }
+            } else {
+                // totals over the row groups, then over the group's items
+                for (int i0 = 0; i0 < (ANY ? S : items); i0 += ANY ? T / LN : T) {
+                    const int i = i0 + (ANY ? t / LN : t);
+                    if (!ANY && i >= items) break;
+                    const int k = kByCol ? 0 : i & 3, q = kByCol ? i : i >> 2;
+                    double s1 = 0.0, s2 = 0.0;
+                    if (ANY) {
+                        if (i < S)
+                            for (int z = t & (LN - 1); z < RT; z += LN) {
+                                s1 += red[k * T + z * CV + q];
+                                s2 += red[(4 + k) * T + z * CV + q];
+                            }
+                        for (int o = LN >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+                        if (i >= S || (t & (LN - 1))) continue;
+                    } else {
+                        for (int z = 0; z < RG; ++z) {
+                            s1 += red[(z * NV + k) * CV + q];
+                            s2 += red[(z * NV + (kByCol ? 1 : 4) + k) * CV + q];
+                        }
+                    }
+                    if (BWD) {
+                        const double *st = a.stats + 2 * ((size_t)ns * a.G + (slab * S + i) / D);
+                        s2 = st[1] * fma((double)gn_centre(st[0], st[1]) - st[0], s1, s2);
+                        if (a.part && n < a.x_batch) { chan[i] += s1; chan[S + i] += s2; }
+                        const double g = (double)a.gamma[slab * S + i];
+                        s1 *= g; s2 *= g;
+                    }
+                    for (int o = DW >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+                    if ((i & (DW - 1)) == 0) {
+                        if (BWD) { stat[i / DW] = s1; stat[S + i / DW] = s2; }
+                        else publish(i / DW, s1, s2);      // (forward: at most 64 items a group)
+                    }
+                }
             }
-        }
+            __syncthreads();
+        };
+        gather(std::true_type());
         if (!BWD) {
+            if (__builtin_expect(*again, 0)) {
+                const float *p2 = px;
+                int r2 = row0;
+                asm volatile("" : "+v"(p2), "+v"(r2));     // (nothing computed for the first reads is kept for these)
+                float pivot[GP];
+#pragma unroll
+                for (int j = 0; j < GP; ++j) pivot[j] = gn_finite(p2[(c0 + j) / D * D - c0]);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) s[k] = 0.0;
+                for (int r = r2; r < HW; r += RT) {
+                    const float4 q = *reinterpret_cast<const float4 *>(p2 + (size_t)r * a.C);
+                    const float xv[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const double d = xv[j] - (double)pivot[j % GP];
+                        s[kByCol ? 0 : j] += d;
+                        s[(kByCol ? 1 : 4 + j) % NV] = fma(d, d, s[(kByCol ? 1 : 4 + j) % NV]);
+                    }
+                }
+                gather(std::false_type());
+            }
+#pragma unroll
+            for (int j = 0; j < GP; ++j) {
+                const int g = (col * 4 + j) / D;
+                rstd[j] = stat[S + g];
+                cf[j] = gn_centre(stat[g], rstd[j]);
+                mean[j] = stat[g] - (double)cf[j];
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) { A[j] = rstd[j % GP] * (double)ga[j]; B[j] = fma(-mean[j % GP], A[j], (double)be[j]); }
-            // one thread per group publishes what its own channels use
-            if (row0 == 0) {
+        } else {
 #pragma unroll
-                for (int j = 0; j < GP; ++j) {
-                    if ((col * 4 + j) % D == 0) {
-                        double *st = a.stats + 2 * ((size_t)n * a.G + g0 + (col * 4 + j) / D);
-                        st[0] = mean[j]; st[1] = rstd[j];
-                    }
+            for (int j = 0; j < GP; ++j) {
+                const int g = (col * 4 + j) / D;
+                if (ANY && j && g == (col * 4 + j - 1) / D) {    // (the same group as the channel before)
+                    L[j] = L[j ? j - 1 : 0]; M[j] = M[j ? j - 1 : 0];
+                    continue;
                 }
+                double s1 = 0.0, s2 = 0.0;
+                for (int q = 0; q < per; ++q) { s1 += stat[g * per + q]; s2 += stat[S + g * per + q]; }
+                s1 *= inv_m; s2 *= inv_m;
+                L[j] = -rstd[j] * rstd[j] * s2;
+                M[j] = -fma(L[j], mean[j], rstd[j] * s1);
             }
         }
         float *po = a.out + (size_t)n * HW * a.C + c0;
@@ -237,6 +315,7 @@ __global__ __launch_bounds__(kGnMaxThreads, gn_waves(U, BWD, TANH, GP)) void gn_
             const int r = row0 + u * RT;
             gn_fresh(vx[u]);
             if (BWD) gn_fresh(vd[BWD ? u : 0]);
+            if (!kOnce) gn_subtract(vx[u], cf[0], cf[1 % GP], cf[2 % GP], cf[3 % GP]);
             const float xv[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
             float dv[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
             if (BWD) { dv[0] = vd[u].x; dv[1] = vd[u].y; dv[2] = vd[u].z; dv[3] = vd[u].w; }
@@ -304,6 +383,7 @@ __global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
     const int p0 = chunk * a.chunk_px;                 // rows are counted from the chunk's first: p0 + chunk_px may pass an int
     const int rows = a.HW - p0 < a.chunk_px ? a.HW - p0 : a.chunk_px;
     double s1[VEC], s2[VEC], mean[VEC], rstd[VEC], ga[VEC], be[VEC];
+    float pivot[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { s1[j] = 0.0; s2[j] = 0.0; }
     if (rl < RT) {
@@ -316,33 +396,71 @@ __global__ __launch_bounds__(256) void gn_partial_kernel(GnArgs a) {
             }
         }
         const float *px = a.x + ((size_t)ns * a.HW + p0) * a.C + c;
-        const float *pd = BWD ? a.dy + ((size_t)n * a.HW + p0) * a.C + c : nullptr;
-        for (int r = rl; r < rows; r += RT * U) {
-            float vx[U][VEC], vd[U][VEC];
+        if (BWD) {
+            const float *pd = a.dy + ((size_t)n * a.HW + p0) * a.C + c;
+            for (int r = rl; r < rows; r += RT * U) {
+                float vx[U][VEC], vd[U][VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int rr = r + u * RT;
-                const bool ok = rr < rows;
-                if (ok) gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
-                if (BWD && ok) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
-                if (!ok) {
+                for (int u = 0; u < U; ++u) {
+                    const int rr = r + u * RT;
+                    const bool ok = rr < rows;
+                    if (ok) gn_load<VEC>(px + (size_t)rr * a.C, vx[u]);
+                    if (ok) gn_load<VEC>(pd + (size_t)rr * a.C, vd[u]);
+                    if (!ok) {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { vx[u][j] = 0.f; vd[u][j] = 0.f; }
+                        for (int j = 0; j < VEC; ++j) { vx[u][j] = 0.f; vd[u][j] = 0.f; }
+                    }
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const double v = vx[u][j];
-                    if (!BWD) { s1[j] += v; s2[j] = fma(v, v, s2[j]); }
-                    else {
-                        const double xh = (v - mean[j]) * rstd[j];
+                    for (int j = 0; j < VEC; ++j) {
+                        const double xh = ((double)vx[u][j] - mean[j]) * rstd[j];
                         const double dz = (double)vd[u][j] * gn_slope<TANH>(fma(xh, ga[j], be[j]), a.below);
                         s1[j] += dz; s2[j] = fma(dz, xh, s2[j]);
                     }
                 }
             }
+        } else {
+            float vx[U][VEC];
+            const int last = rows - 1;
+            auto fetch = [&](int r) {                      // (a row beyond the chunk: its last row again)
+#pragma unroll
+                for (int u = 0; u < U; ++u) gn_load<VEC>(px + (size_t)(r + u * RT < last ? r + u * RT : last) * a.C, vx[u]);
+            };
+            int r = rl, g = sl.groups == 1 ? sl.g0 : c / a.D, f = g * a.D;     // the channel's group and that one's first channel
+            fetch(r);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {                // (in flight beside the first rows)
+                if (c + j == f + a.D) f += a.D;
+                pivot[j] = a.x[(size_t)n * a.HW * a.C + f];
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) pivot[j] = gn_finite(pivot[j]);
+            if (chunk == 0 && rl == 0) {                   // (kept for the second pass, which may write where x stands)
+                f = g * a.D;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (c + j == f + a.D) { f += a.D; ++g; }
+                    if (c + j == f) a.pivot[(size_t)n * a.G + g] = pivot[j];
+                }
+            }
+            auto add = [&](int u) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const double d = (double)vx[u][j] - (double)pivot[j];
+                    s1[j] += d; s2[j] = fma(d, d, s2[j]);
+                }
+            };
+            while (r + (U - 1) * RT < rows) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) add(u);
+                r += RT * U;
+                fetch(r);
+            }
+#pragma unroll
+            for (int u = 0; u < U - 1; ++u)
+                if (r + u * RT < rows) add(u);
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -390,10 +508,10 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
     const int rows = a.HW - p0 < a.chunk_px ? a.HW - p0 : a.chunk_px;
     const int P = a.chunks * a.pieces;
     const double inv_m = 1.0 / ((double)a.HW * a.D);
-    auto publish = [&](int g, double u1, double u2) {
+    auto publish = [&](int g, double u1, double u2, double pivot) {
         if (BWD) { stat[0][g] = u1 * inv_m; stat[1][g] = u2 * inv_m; return; }
-        const double mu = u1 * inv_m;
-        double var = u2 * inv_m - mu * mu;
+        const double off = u1 * inv_m, mu = pivot + off;
+        double var = fma(-off, off, u2 * inv_m);
         if (var < 0.0) var = 0.0;
         const double is = 1.0 / sqrt(var + (double)a.eps);
         stat[0][g] = mu; stat[1][g] = is;
@@ -416,17 +534,19 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
     };
     fetch(rl);                                         // in flight while the statistics come together
     const int lanes = gn_lanes(sl.groups), mine = t / lanes, l = t & (lanes - 1);
-    double u1 = 0.0, u2 = 0.0;
+    double u1 = 0.0, u2 = 0.0, pivot = 0.0;
     if (mine < sl.groups) {
+        if (!BWD) pivot = a.pivot[(size_t)n * a.G + sl.g0 + mine];
         const double2 *q = reinterpret_cast<const double2 *>(a.gpart + ((size_t)n * a.G + sl.g0 + mine) * P * 2);
 #pragma unroll 4
         for (int p = l; p < P; p += lanes) { const double2 v = q[p]; u1 += v.x; u2 += v.y; }
     }
     for (int o = lanes >> 1; o > 0; o >>= 1) { u1 += __shfl_xor(u1, o, 64); u2 += __shfl_xor(u2, o, 64); }
-    if (mine < sl.groups && l == 0) publish(mine, u1, u2);
+    if (mine < sl.groups && l == 0) publish(mine, u1, u2, pivot);
     __syncthreads();
     if (rl >= RT) return;
     double A[VEC], B[VEC], L[VEC], M[VEC];             // the maps of the resident form
+    float cf[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const int g = (c + j) / a.D - sl.g0;
@@ -434,10 +554,14 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
         if (BWD) {
             const double *st = a.stats + 2 * ((size_t)ns * a.G + sl.g0 + g);
             mean = st[0]; rstd = st[1];
-            L[j] = -rstd * rstd * stat[1][g];
-            M[j] = -fma(L[j], mean, rstd * stat[0][g]);
         } else {
             mean = stat[0][g]; rstd = stat[1][g];
+        }
+        cf[j] = gn_centre(mean, rstd);
+        mean -= (double)cf[j];
+        if (BWD) {
+            L[j] = -rstd * rstd * stat[1][g];
+            M[j] = -fma(L[j], mean, rstd * stat[0][g]);
         }
         A[j] = rstd * (double)a.gamma[c + j];
         B[j] = fma(-mean, A[j], (double)a.beta[c + j]);
@@ -451,7 +575,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a) {
             float o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const double v = vx[u][j], z = fma(A[j], v, B[j]);
+                const double v = vx[u][j] - cf[j], z = fma(A[j], v, B[j]);
                 if (!BWD) o[j] = gn_act<TANH>((float)z, a.below);
                 else o[j] = (float)fma(A[j], (double)vd[BWD ? u : 0][j] * gn_slope<TANH>(z, a.below), fma(L[j], v, M[j]));
             }
@@ -562,7 +686,7 @@ static size_t gn_bytes(long N, long HW, int C, int G) {
     GnPlan p;
     gn_plan_split(HW, C, C / G, N, p);
     const size_t gpart = (size_t)N * G * p.chunks * p.pieces * 2 * sizeof(double);
-    size_t part = (size_t)N * p.chunks * 2 * C * sizeof(double);
+    const size_t part = (size_t)N * p.chunks * 2 * C * sizeof(double);      // (forward: N G first values in its place)
     return gpart + part + 256;
 }
 
@@ -600,15 +724,20 @@ static int gn_run(GnArgs &a, float *dgamma, float *dbeta, void *workspace, hipSt
         a.rows = (int)gn_resident_rows(a.N, a.slabs);
         part_rows = a.rows;
         a.part = params ? (double *)workspace : nullptr;
-        if (p.any) gn_launch_resident<BWD, TANH, 4, true>(a, p, st);
-        else if (a.D % 4 == 0) gn_launch_resident<BWD, TANH, 1, false>(a, p, st);
+        if (p.any) {
+            if constexpr (BWD) gn_launch_resident<true, TANH, 4, true>(a, p, st);            // (per channel: dgamma, dbeta)
+            else if (a.D % 4 == 0) gn_launch_resident<false, TANH, 1, true>(a, p, st);
+            else gn_launch_resident<false, TANH, 4, true>(a, p, st);
+        } else if (a.D % 4 == 0) gn_launch_resident<BWD, TANH, 1, false>(a, p, st);
         else gn_launch_resident<BWD, TANH, 4, false>(a, p, st);
     } else {
         gn_plan_split(a.HW, a.C, a.D, a.N, p);
         a.SB = p.SB; a.gps = p.gps; a.pieces = p.pieces; a.slabs = p.slabs; a.chunks = p.chunks; a.chunk_px = p.chunk_px;
         a.gpart = (double *)workspace;
         part_rows = (long)a.x_batch * a.chunks;
-        a.part = params ? a.gpart + (size_t)a.N * a.G * a.chunks * a.pieces * 2 : nullptr;
+        double *rest = a.gpart + (size_t)a.N * a.G * a.chunks * a.pieces * 2;
+        a.pivot = BWD ? nullptr : rest;
+        a.part = params ? rest : nullptr;
         const bool vec = !(a.C & 3) && (a.pieces == 1 ? !(a.SB & 3) : !(a.D & 3)) && gn_aligned(a.x) && gn_aligned(a.out) && (!BWD || gn_aligned(a.dy));
         const dim3 grid(p.slabs, p.chunks, a.N), block(256);
         if (vec) {
