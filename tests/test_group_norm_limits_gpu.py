@@ -58,8 +58,13 @@ def test_the_largest_image(ops, HW, C, G):
 
 
 def test_many_one_channel_groups(ops):
-    """2^22 - 1 groups of one value: each is its own mean, y = beta"""
+    """2^22 - 1 groups of one value: each is its own mean, and y is beta but for A x + B = rstd gamma x + (beta - rstd gamma x): B and the sum
+    are rounded to 64 bits, 2^-53 of |beta| + |rstd gamma x| each (|x| rstd being at most 256 where B is not taken around x itself), before
+    one rounding to 32"""
     C = (1 << 22) - 1
-    x, gamma, beta = (torch.randn(C, device='cuda') for _ in range(3))
+    g = torch.Generator(device='cuda').manual_seed(3)
+    x, gamma, beta = (torch.randn(C, device='cuda', generator=g) for _ in range(3))
     y, stats = ops.group_norm_fwd(x.view(1, 1, C), gamma, beta, C)
-    assert torch.equal(y.view(-1), beta) and torch.equal(stats[0, :, 0], x.double())
+    assert torch.equal(stats[0, :, 0], x.double())
+    b = beta.double().abs()
+    assert ((y.view(-1).double() - beta.double()).abs() <= U * b + 2 * 2.0 ** -53 * (b + 256 * gamma.double().abs())).all()
