@@ -366,6 +366,7 @@ int mmdgan_bn_bwd(const float *x, const float *y, const float *dy, long rows, in
  * Unlike batch norm the rows stay independent and there are no moving statistics: inference is the forward call.
  * workspace: mmdgan_gn_workspace_bytes(N, HW, C, G) bytes of device scratch, 16-byte aligned, nothing kept in it between
  * calls (two calls that may overlap in time need one each).  Sums in a fixed order: equal inputs give equal bits.
+ * A group that holds an infinity or NaN is NaN in y under every activation (batch norm's relu maps NaN to 0) and in dx.
  * 16-byte aligned tensors with C % 4 == 0 get the float4 kernels, others scalar ones.  N <= 65535, HW * C < 2^31.
  * (The reference has batch norm only, layer_func.py:955-966: 'act_nm': 'gn' is this library's addition.)
  * ---------------------------------------------------------------------------------------------- */

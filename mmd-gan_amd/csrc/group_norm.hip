@@ -42,11 +42,12 @@ struct GnArgs {
     int SB, gps, pieces, chunks, chunk_px;
 };
 
-// The activation by its side below zero: 0 relu, 0.1 lrelu, 1 linear (common.h: act_fwd, the same value for every input, NaN
-// included); tanh is a template argument of the kernels - its code in every unrolled element costs registers the others need.
+// The activation by its side below zero: 0 relu, 0.1 lrelu, 1 linear (common.h: act_fwd, the same value for every number; NaN stays NaN
+// under relu too, so that an image whose statistics are spoiled shows in y as it does in dx); tanh is a template argument of the
+// kernels - its code in every unrolled element costs registers the others need.
 template <bool TANH> __device__ __forceinline__ float gn_act(float z, float below) {
     if (TANH) return tanhf(z);
-    return z > 0.f ? z : below == 0.f ? 0.f : z * below;
+    return !(z <= 0.f) ? z : below == 0.f ? 0.f : z * below;
 }
 template <bool TANH> __device__ __forceinline__ double gn_slope(double z, float below) {
     if (TANH) {

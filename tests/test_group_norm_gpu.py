@@ -284,3 +284,23 @@ def test_a_workspace_is_real_memory(ops):
         ops.group_norm_fwd(x, v, v, 3, workspace=fake)
     with pytest.raises(AssertionError, match='workspace'):
         ops.group_norm_bwd(x, x, v, v, st, workspace=fake)
+
+
+@pytest.mark.parametrize('N,HW,C,G', [(4, 40, 16, 4), (4, 40, 16, 16), (3, 50, 60, 12), (3, 35, 15, 5), (2, 3000, 12, 4)])
+def test_a_bad_image_shows_under_every_activation(ops, N, HW, C, G):
+    """a group that holds an infinity or NaN is NaN in y whatever the activation (relu of NaN is NaN), as in dx; the other groups and images
+    keep their bits"""
+    x, gamma, beta, dy = (t.cuda() for t in data(N, HW, C, 41))
+    D = C // G
+    for act in ('linear', 'relu', 'lrelu', 'tanh'):
+        y0, st0 = ops.group_norm_fwd(x, gamma, beta, G, act=act)
+        dx0, _, _ = ops.group_norm_bwd(x, dy, gamma, beta, st0, act=act)
+        for bad in (float('nan'), float('inf'), float('-inf')):
+            x2 = x.clone()
+            x2[1, HW // 2, D] = bad                              # image 1, group 1
+            y, st = ops.group_norm_fwd(x2, gamma, beta, G, act=act)
+            dx, _, _ = ops.group_norm_bwd(x2, dy, gamma, beta, st, act=act)
+            spoiled = torch.zeros_like(y, dtype=torch.bool)
+            spoiled[1, :, D:2 * D] = True
+            assert torch.equal(torch.isnan(y), spoiled) and torch.equal(torch.isnan(dx), spoiled), (act, bad)
+            assert torch.equal(y[~spoiled], y0[~spoiled]) and torch.equal(dx[~spoiled], dx0[~spoiled])
