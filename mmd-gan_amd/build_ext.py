@@ -2,7 +2,7 @@
 """Build libmmdgan_hip.so (gfx950) in-tree: mmd-gan_amd/lib/libmmdgan_hip.so.
 
 hipcc cross-compiles without a GPU.  Objects are rebuilt only when their source (or a header)
-is newer.  Usage: python mmd-gan_amd/build_ext.py [--force]
+is newer, or when they were built with another compiler or other flags.  Usage: python mmd-gan_amd/build_ext.py [--force]
 """
 import concurrent.futures
 import glob
@@ -35,6 +35,11 @@ def build(force=False, verbose=True):
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, '*.hip')))
     hdrs = sorted(glob.glob(os.path.join(CSRC, '*.h'))) + [os.path.join(HERE, '..', 'include', 'mmdgan_hip.h')]
+    stamp, how = os.path.join(OBJ, 'flags.txt'), ' '.join([HIPCC] + FLAGS)
+    if not os.path.exists(stamp) or open(stamp).read() != how:
+        force = True
+    if force and os.path.exists(stamp):
+        os.remove(stamp)                                 # (back when every object is of these flags)
     jobs = []
     for s in srcs:
         o = os.path.join(OBJ, os.path.basename(s)[:-4] + '.o')
@@ -60,6 +65,8 @@ def build(force=False, verbose=True):
         if r.returncode != 0:
             sys.stderr.write(r.stderr)
             raise RuntimeError('link failed')
+        with open(stamp, 'w') as f:
+            f.write(how)
     return LIB
 
 
