@@ -74,3 +74,25 @@ def test_the_driver_entry_compiles_every_time(monkeypatch):
     monkeypatch.setattr(build_ext, 'build', lambda force=False, verbose=True: calls.append(force) or build_ext.LIB)
     g.build()
     assert calls == [True]
+
+
+def test_no_device_code_is_compiled_with_packed_fp32():
+    """every compiler line for gfx950 that names a .hip source carries the flag, the tools' too, and none writes packed fp32 by hand"""
+    import glob
+    import re
+    flag, found = '-packed-fp32-ops', 0
+    files = [f for p in ('tools/*', 'mmd-gan_amd/*.py', 'oracle/*.py', '*.py') for f in glob.glob(os.path.join(ROOT, p)) if os.path.isfile(f)]
+    for f in files:
+        if not f.endswith(('.sh', '.py', '.hip', '.md')):
+            continue
+        pieces = re.split(r'--offload-arch=gfx950', open(f).read())
+        for piece in pieces[1:]:
+            if re.search(r'\.hip\b', piece[:600].split('\n\n')[0]):
+                found += 1
+                assert flag in piece[:600], (f, piece[:200])
+    assert found >= 14
+    import build_ext
+    assert flag in build_ext.FLAGS
+    for f in glob.glob(os.path.join(ROOT, 'tools', '*.hip')) + glob.glob(os.path.join(ROOT, 'mmd-gan_amd', 'csrc', '*')):
+        text = re.sub(r'//[^\n]*', '', open(f).read())
+        assert not re.search(r'v_pk_(add|mul|fma)_f32', text), f

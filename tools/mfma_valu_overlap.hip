@@ -1,11 +1,11 @@
 // Do a consumer wave's MFMAs and a producer wave's VALU work overlap when the two waves share a SIMD (8-wave workgroup, waves
 // 0-3 MFMA-only, waves 4-7 VALU-only)?  One workgroup per CU on every CU; times of: MFMAs alone, VALU alone (plain fp32 FMAs /
-// packed v_pk_fma_f32 / ds_write_b64), and both.   hipcc -O3 --offload-arch=gfx950 tools/mfma_valu_overlap.hip -o tools/scratch/mvo.bin
+// ds_write_b64), and both.   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_valu_overlap.hip -o tools/scratch/mvo.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <int MODE, int VKIND>   // MODE bit 0: MFMAs, bit 1: VALU work;  VKIND 0 fma, 1 pk_fma, 2 ds_write_b64 + fma mix
+template <int MODE, int VKIND>   // MODE bit 0: MFMAs, bit 1: VALU work;  VKIND 0 fma, 2 ds_write_b64 + fma mix, 3-5 fma in 2 / 4 / 6 dependent chains
 __global__ __launch_bounds__(512) void k(float *out, int iters) {
     __shared__ float lds[8192];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -30,26 +30,13 @@ __global__ __launch_bounds__(512) void k(float *out, int iters) {
             for (int e = 0; e < 16; ++e) v[e] = lane + e;
             for (int it = 0; it < iters; ++it) {
 #pragma unroll
-                for (int rep = 0; rep < 24; ++rep)          // 384 plain FMAs per iteration (= 192 packed)
+                for (int rep = 0; rep < 24; ++rep)          // 384 FMAs per iteration
 #pragma unroll
                     for (int e = 0; e < 16; ++e) v[e] = fmaf(v[e], 1.0001f, 0.5f);
             }
             float s = 0;
             for (int e = 0; e < 16; ++e) s += v[e];
             if (s == 1.2345f) out[threadIdx.x] = s;
-        } else if (VKIND == 1) {
-            f32x2 v[16];
-            for (int e = 0; e < 16; ++e) v[e] = f32x2{(float)lane + e, (float)e};
-            const f32x2 c1 = {1.0001f, 1.0001f}, c2 = {0.5f, 0.5f};
-            for (int it = 0; it < iters; ++it) {
-#pragma unroll
-                for (int rep = 0; rep < 12; ++rep)          // 192 packed FMAs per iteration
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = __builtin_elementwise_fma(v[e], c1, c2);
-            }
-            f32x2 s = {0, 0};
-            for (int e = 0; e < 16; ++e) s += v[e];
-            if (s.x + s.y == 1.2345f) out[threadIdx.x] = s.x;
         } else if (VKIND >= 3 && VKIND <= 5) {
             constexpr int NCH = VKIND == 3 ? 2 : VKIND == 4 ? 4 : 6;
             float v[NCH];
@@ -88,15 +75,13 @@ template <int MODE, int VKIND> float run(float *out, int iters) {
 }
 int main() {
     float *out; (void)hipMalloc(&out, 4096);
-    const int iters = 200;   // per iteration: 36 MFMAs (2304 cycles of the matrix pipe) | 384 FMAs | 192 packed FMAs | 36 LDS stores
+    const int iters = 200;   // per iteration: 36 MFMAs (2304 cycles of the matrix pipe) | 384 FMAs | 36 LDS stores
     printf("per iteration: 36 x v_mfma_f32_32x32x2_f32 on waves 0-3, VALU work on waves 4-7; %d iterations, us per launch (cycles per iteration at 2.4 GHz)\n", iters);
     auto cyc = [&](float us) { return us * 2400.f / iters; };
     float m = run<1, 0>(out, iters);
     printf("MFMAs alone                      %8.1f us (%6.0f)\n", m, cyc(m));
     float a0 = run<2, 0>(out, iters), b0 = run<3, 0>(out, iters);
     printf("384 v_fma_f32: alone %8.1f us (%6.0f)   with the MFMAs %8.1f us (%6.0f)\n", a0, cyc(a0), b0, cyc(b0));
-    float a1 = run<2, 1>(out, iters), b1 = run<3, 1>(out, iters);
-    printf("192 v_pk_fma_f32: alone %8.1f us (%6.0f)   with the MFMAs %8.1f us (%6.0f)\n", a1, cyc(a1), b1, cyc(b1));
     float a2 = run<2, 2>(out, iters), b2 = run<3, 2>(out, iters);
     printf("36 ds_write_b64: alone %8.1f us (%6.0f)   with the MFMAs %8.1f us (%6.0f)\n", a2, cyc(a2), b2, cyc(b2));
     float a3 = run<2, 3>(out, iters), b3 = run<3, 3>(out, iters);

@@ -14,7 +14,7 @@ declare -A V=(
 )
 if [ "$1" = build ]; then
   for k in "${!V[@]}"; do
-    hipcc -w -O3 --offload-arch=gfx950 -I../include ${V[$k]} -DVARIANT="\"$k\"" igemm_probe.hip -o probe_$k.bin &
+    hipcc -w -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -I../include ${V[$k]} -DVARIANT="\"$k\"" igemm_probe.hip -o probe_$k.bin &
   done
   wait
 else

@@ -15,7 +15,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path[:0] = [os.path.join(ROOT, 'mmd-gan_amd'), ROOT]
 so = os.path.join(ROOT, 'tools', 'libclockprobe.so')
 if not os.path.exists(so):
-    subprocess.check_call(['/opt/rocm/bin/hipcc', '-O3', '--offload-arch=gfx950', '-shared', '-fPIC',
+    subprocess.check_call(['/opt/rocm/bin/hipcc', '-O3', '--offload-arch=gfx950', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-shared', '-fPIC',
                            os.path.join(ROOT, 'tools', 'clock_probe.hip'), '-o', so])
 lib = ctypes.CDLL(so)
 lib.clock_probe.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

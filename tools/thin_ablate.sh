@@ -8,7 +8,7 @@ MASKS="0 1 2 4 3 7"
 if [ "$1" = build ]; then
     mkdir -p $R/tools/scratch/thinlibs && cd $R/mmd-gan_amd && python build_ext.py > /dev/null || exit 1
     for m in $MASKS; do
-        /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -DTHIN_ABLATE=$m -c csrc/conv_thin_mfma.hip -o /tmp/thin_$m.o &&
+        /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -Wno-unused-function -DTHIN_ABLATE=$m -c csrc/conv_thin_mfma.hip -o /tmp/thin_$m.o &&
         /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/tools/scratch/thinlibs/lib_$m.so $(ls build/*.o | grep -v conv_thin_mfma.o) /tmp/thin_$m.o || exit 1
     done
     exit 0

@@ -4,7 +4,7 @@
 //   dword  x 2 runs of 128 B     (csrc/conv_wino43w.hip, second cut)      b64 x 4 runs of 128 B   (shipped)
 //   b128   x 8 runs of 128 B                                               b128 x 1 run of 1 KB / dword x 1 run of 256 B (contiguous)
 // The working set per workgroup is a few hundred KB walked repeatedly (L2 hits), or `big` = a stride that defeats the L2.
-//   hipcc -O3 --offload-arch=gfx950 tools/vmem_request_rate.hip -o tools/scratch/vrr.bin
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/vmem_request_rate.hip -o tools/scratch/vrr.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

@@ -1,5 +1,5 @@
 // where do the workgroups of a 2-per-CU persistent grid land?  prints, per (XCC, SE, CU), the wave slots / SIMDs of the first
-// wave of every resident workgroup.  hipcc -O3 --offload-arch=gfx950 wg_census.hip -o wg_census.bin
+// wave of every resident workgroup.  hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops wg_census.hip -o wg_census.bin
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <map>

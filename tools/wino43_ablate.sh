@@ -11,7 +11,7 @@ if [ "$1" = build ]; then
     mkdir -p $R/tools/scratch/w43libs && cd $R/mmd-gan_amd && python build_ext.py > /dev/null || exit 1
     rm -f $R/tools/scratch/w43libs/*.so
     for m in $MASKS; do
-        ( /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -Wno-unused-value -DW43_ABLATE=$m -c csrc/conv_wino43.hip -o /tmp/w43_$m.o &&
+        ( /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -Wno-unused-function -Wno-unused-value -DW43_ABLATE=$m -c csrc/conv_wino43.hip -o /tmp/w43_$m.o &&
           /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/tools/scratch/w43libs/lib_$m.so $(ls build/*.o | grep -v conv_wino43.o) /tmp/w43_$m.o || echo "mask $m failed" ) &
         [ $(jobs -r | wc -l) -ge 6 ] && wait -n
     done

@@ -16,7 +16,7 @@ if sys.argv[1:2] == ['build']:
     os.makedirs(os.path.dirname(TRACE), exist_ok=True)
     os.chdir(os.path.join(ROOT, 'mmd-gan_amd'))
     subprocess.check_call([sys.executable, 'build_ext.py'], stdout=subprocess.DEVNULL)
-    subprocess.check_call('/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -Wno-unused-value -DW43W_TRACE=%s '
+    subprocess.check_call('/opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -Wno-unused-function -Wno-unused-value -DW43W_TRACE=%s '
                           '%s -c csrc/conv_wino43w.hip -o /tmp/w43w_trace.o && /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o %s '
                           '$(ls build/*.o | grep -v conv_wino43w.o) /tmp/w43w_trace.o' % (sys.argv[2] if len(sys.argv) > 2 else '17', ' '.join(sys.argv[3:]), TRACE), shell=True)
     sys.exit(0)
