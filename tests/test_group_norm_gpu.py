@@ -304,3 +304,22 @@ def test_a_bad_image_shows_under_every_activation(ops, N, HW, C, G):
             spoiled[1, :, D:2 * D] = True
             assert torch.equal(torch.isnan(y), spoiled) and torch.equal(torch.isnan(dx), spoiled), (act, bad)
             assert torch.equal(y[~spoiled], y0[~spoiled]) and torch.equal(dx[~spoiled], dx0[~spoiled])
+
+
+@pytest.mark.parametrize('N,HW,C,G', [(3, 65, 48, 12), (2, 1023, 32, 8), (3, 64, 32, 32), (3, 50, 60, 12), (2, 33, 15, 5), (2, 9000, 4, 4), (33, 1457, 96, 32)])
+def test_tanh_backward_within_its_own_error(ops, N, HW, C, G):
+    """the slope is 4 e / (1 + e)^2 with e = exp(-2 |z|) in 32 bits.  e: (2 + 6 |z|) u (the exponential's last place is 2 u; z, the constant and
+    their product u each, of 2 |z|), of which tanh |z| counts, times the slope 1 / cosh^2 z: at most 2.6 u.  1 + e: u, its reciprocal 2 u, both
+    squared, and two products: 8 u of the slope.  Together at most 9 u of 1; dz itself stays in 64 bits.  So dx is within u of itself and 9 u
+    of each term |rstd gamma dy| (2 + |xhat|), and the parameters' sums within 9 u of theirs."""
+    x, gamma, beta, dy = data(N, HW, C, 51 + C)
+    _, stats = ops.group_norm_fwd(x.cuda(), gamma.cuda(), beta.cuda(), G, act='tanh')
+    dx, dgamma, dbeta = ops.group_norm_bwd(x.cuda(), dy.cuda(), gamma.cuda(), beta.cuda(), stats, act='tanh')
+    rx, rg, rb, terms, dz, xhat = backward64(x.double(), dy.double(), gamma.double(), beta.double(), G, 'tanh')
+    z = torch.linspace(0, 20, 1 << 16, dtype=torch.float64)
+    assert float(((2 + 6 * z) * torch.tanh(z) / torch.cosh(z) ** 2 + 8 / torch.cosh(z) ** 2).max()) <= 9
+    slack = 9 * U
+    assert ((dx.cpu().double() - rx).abs() <= U * rx.abs() + (slack + 1e-11) * terms).all()
+    a = dy.double().abs()
+    assert ((dgamma.cpu().double() - rg).abs() <= U * rg.abs() + (slack + 1e-11) * (a * xhat.abs()).sum(dim=(0, 1))).all()
+    assert ((dbeta.cpu().double() - rb).abs() <= U * rb.abs() + (slack + 1e-11) * a.sum(dim=(0, 1))).all()
