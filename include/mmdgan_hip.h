@@ -526,7 +526,9 @@ int mmdgan_adam_prepare_multi(const mmdgan_adam_prepare_job *jobs, int n, void *
  *                  out = (1 - lr * weight_decay) * param - lr * 0.2 * sqrt(max(rows, cols)) * O
  *                  - the factor gives every matrix an update of root mean square 0.2 lr, an Adam step's size, so that one learning
  *                  rate serves a net whose vectors stay with Adam.  out may be param, momentum_out may be momentum.
- * Results are as near to the exact ones as 32-bit products on X give, for ill-conditioned and rank-deficient U too; sums in a fixed
+ * (a, b, c): K. Jordan, Muon, 2024; the factor 0.2 sqrt(max(rows, cols)): J. Liu et al., 2025.
+ * Results are about as near to the exact ones as 32-bit products on X give, for ill-conditioned and rank-deficient U and at every
+ * step count too (operands of 22 bits, sums in 32 and 64; with a side of 64 or less 64 bits throughout); sums in a fixed
  * order: equal inputs give equal bits (replicas of a data-parallel job stay identical).  All matrices of a call run
  * together, phase by phase, 16 at a time: 21 launches at five steps for those with both sides above 64, 3 per eight steps for the
  * others (in 64 bits: csrc/muon_small.hip).  jobs: HOST array, read during the call.  What a matrix writes may overlap nothing of the call but

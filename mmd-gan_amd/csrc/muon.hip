@@ -1,6 +1,7 @@
 // Orthogonalised updates: O = the fifth (or any) iterate of the quintic  X <- a X + b (X X^T) X + c (X X^T)^2 X  started at
 // X = U / ||U||_F, which takes every singular value of U to about 1 (0.7 .. 1.2), and the parameter update that applies it
-// to a momentum matrix.  Matrices are row-major [rows, cols]; m = the shorter side, n = the longer one, X is [m, n].
+// to a momentum matrix.  (a, b, c) = (3.4445, -4.7750, 2.0315) and the method are K. Jordan's (Muon, 2024); the step's factor
+// 0.2 sqrt(max(rows, cols)), which gives every matrix an Adam update's size, is J. Liu et al.'s (2025).  Matrices are row-major [rows, cols]; m = the shorter side, n = the longer one, X is [m, n].
 //
 // Mathematics used.  With A = X X^T the iterate is X' = Q X, Q = a I + b A + c A^2, and the next Gram matrix is
 // A' = Q A Q: all of them are polynomials of one symmetric matrix, they commute, so up to three steps run on m x m
@@ -12,7 +13,8 @@
 // Numerics.  Every m x n and m x m operand is held as TWO fp16 numbers, v * s = hi + lo with s a fixed power of two that keeps
 // the largest possible entry (the norms are bounded: singular values <= 1.21, |Q| <= 3.45, |P| <= 41) below 65504: 22 bits, and
 // 2^-25 / s absolute where lo underflows.  Products are hi hi + hi lo + lo hi in fp32 accumulators (lo lo is 2^-22 of the
-// result): as good as fp32 operands at 16/3 of the fp32 matrix rate.
+// result): operands of 22 bits where fp32's have 24, at 16/3 of the fp32 matrix rate.  What comes out is about as near to 64 bits as fp32
+// products on X: 4608x512 3.3e-6 against 5.7e-6, 129x1001 5.2e-6 and 5.5e-6; an update may be a tenth further off at other sizes.
 //
 // Layout ("packed"): an [R, K] operand is cut into 32 x 16 blocks, row blocks outermost; a block is 2 KB: the 64 lanes' 16-byte
 // MFMA operands of the hi parts in lane order (lane = row % 32 + 32 * (k / 8 % 2), 8 halves along k), then those of the lo parts.
@@ -22,8 +24,9 @@
 // otherwise read addresses that are equal modulo 128 KB, from the same few memory channels.
 //
 // Measured (five steps; 21 launches): 4608x512 alone 147 us - thirteen m x m products of 5.5 us, latency, not work (24 us at the rate of
-// a large fp16 product); the 64x64 images' discriminator (24 M parameters) 0.92 ms: momentum and norm 92 us and the split 47 (HBM),
-// two Gram matrices 92 + 21 each (0.6 of a large product's rate), thirteen m x m products of 21, two products with X 163 and 178 (0.67).
+// a large fp16 product); the 64x64 images' discriminator (24 M parameters) 0.92 to 0.98 ms over several boxes: momentum and norm 92 us and
+// the split 47 (HBM), two Gram matrices 91 + 20 each (0.6 of a large product's rate), thirteen m x m products of 20, two products with X
+// 166 and 181 (0.67).
 #include "muon_internal.h"
 
 namespace mmdgan {
@@ -38,8 +41,8 @@ typedef unsigned int mu_u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMuPad = 128;
 constexpr int kMuChain = 3;                  // steps between two true Gram matrices
 // X <- P X in tiles of 128 x 128; of 64 x 128 where a launch has fewer than 512 of the former (two on a CU at once): 129x1001
-// alone 131 -> 119 us, 4608x512 171 -> 163.  On a net's matrices together the finer tiles change nothing or cost: they read half
-// as much again per product (64x64 images' discriminator 0.99 -> 1.00 ms).
+// alone 131 -> 119 us, 4608x512 171 -> 163 when this was taken (102 and 147 with what came later).  On a net's matrices together the
+// finer tiles change nothing or cost: they read half as much again per product (64x64 images' discriminator 0.99 -> 1.00 ms).
 constexpr int kMuApplyFine = 512;
 constexpr float kScaleX = 4096.f, kScaleA = 4096.f, kScaleQ = 8192.f, kScaleP = 1024.f;
 
