@@ -40,6 +40,9 @@ typedef unsigned int mu_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMuPad = 128;
 constexpr int kMuChain = 3;                  // steps between two true Gram matrices
+// ... but three steps alone run as two and one: a chain of three is off by up to 3.3e-5 on a matrix of rank one (66x271), which the steps before
+// or behind it make nothing of (five steps: 4.4e-5, on X itself 5.3e-5) and which three steps on X itself, 4.5e-6, do not have.
+static int mu_chain(int done, int steps) { return steps == 3 && done == 0 ? 2 : steps - done < kMuChain ? steps - done : kMuChain; }
 // X <- P X in tiles of 128 x 128; of 64 x 128 where a launch has fewer than 512 of the former (two on a CU at once): 129x1001
 // alone 131 -> 119 us, 4608x512 171 -> 163 when this was taken (102 and 147 with what came later).  On a net's matrices together the
 // finer tiles change nothing or cost: they read half as much again per product (64x64 images' discriminator 0.99 -> 1.00 ms).
@@ -602,7 +605,7 @@ static MuMat mu_place(int rows, int cols, bool keep_u, int steps, size_t base) {
     m.part = take((size_t)m.nparts * sizeof(double));
     m.u = keep_u ? take((size_t)n * 4) : 0;
     m.x = take(bx); m.xt = take(bt);
-    m.xt2 = steps > kMuChain ? take(bt) : 0;
+    m.xt2 = steps > mu_chain(0, steps) ? take(bt) : 0;
     m.a = take(sq); m.qq = take(sq); m.w = take(sq); m.p0 = take(sq); m.p1 = take(sq);
     m.slab = take((size_t)m.splits * m.tiles * 128 * 128 * 4);
     m.end = o;
@@ -667,7 +670,7 @@ static void mu_run_group(const MuJob *jobs, int n, bool update, const MuStep &sp
         hipLaunchKernelGGL(mu_split_kernel, dim3(blocks), dim3(256), 0, st, t);
     }
     for (int done = 0; done < steps;) {
-        const int chain = steps - done < kMuChain ? steps - done : kMuChain;
+        const int chain = mu_chain(done, steps);
         {
             MuGramTable t{};
             unsigned blocks = 0, red = 0;

@@ -14,7 +14,7 @@ import math
 import pytest
 import torch
 
-from test_muon_gpu import A, B, C, make
+from test_muon_gpu import A, B, C, make, orth64, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,17 @@ def test_many_steps_in_place_in_a_graph_and_with_foreign_scratch(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize('steps', [1, 2, 3, 4, 6, 7])
+def test_few_steps_on_matrices_of_every_kind(ops, steps):
+    """against the definition at test_muon_gpu.py's bar, a score of matrices of each kind: the bar is tight at few steps, where nothing has been
+    stretched yet, and rank-one matrices with a long side come nearest to it"""
+    for rows, cols in ((66, 271), (4000, 70), (129, 300), (40, 300)):
+        for kind in KINDS:
+            us = [make(kind, rows, cols, seed) for seed in [48244] + list(range(1000 * steps, 1000 * steps + 20))]
+            outs = ops.orthogonalize([u.cuda() for u in us], steps=steps)
+            for u, o in zip(us, outs):
+                ref = orth64(u, steps)
+                err, bar = float((o.cpu().double() - ref).norm()), tolerance(u, ref, steps)
+                assert err <= bar, (rows, cols, kind, err, bar)
