@@ -149,10 +149,10 @@ __global__ __launch_bounds__(w43::NT) void wino43_kernel(int N, int H, int W, in
         __builtin_amdgcn_s_setprio(W43_PRODUCER_PRIO);
 #endif
         // ---------------------------------------------------------------- producers: patches -> B^T d B -> V
-        // lane of the four waves = (tile, channel PAIR of the window's 16): everything below works on f32x2 (two
-        // channels side by side: one 8-byte load and store for both; no packed arithmetic, the library is built without it).  With the stage's channel c on k half (c >> 1) & 1, k-pair (c & 1) +
-        // 2 (c >> 2) - the order wino43_weight_block lays U out in - a pair is two consecutive k-pairs of one k half: one
-        // 8-byte store of V per frequency.
+        // lane of the four waves = (tile, channel PAIR of the window's 16): everything below works on f32x2 (two channels side by
+        // side: one 8-byte load and store for both; no packed arithmetic, the library is built without it).  With the stage's
+        // channel c on k half (c >> 1) & 1, k-pair (c & 1) + 2 (c >> 2) - the order wino43_weight_block lays U out in - a pair is
+        // two consecutive k-pairs of one k half: one 8-byte store of V per frequency.
         const int pl = (wave - 4) * 64 + lane, pt = pl >> 3, cp = pl & 7, sub = cp >> 2, pkh = cp & 1, pkp = cp & 2;
         unsigned rowb[6], colb[6];
         {

@@ -1,13 +1,14 @@
 // Orthogonalised updates: O = the fifth (or any) iterate of the quintic  X <- a X + b (X X^T) X + c (X X^T)^2 X  started at
 // X = U / ||U||_F, which takes every singular value of U to about 1 (0.7 .. 1.2), and the parameter update that applies it
 // to a momentum matrix.  (a, b, c) = (3.4445, -4.7750, 2.0315) and the method are K. Jordan's (Muon, 2024); the step's factor
-// 0.2 sqrt(max(rows, cols)), which gives every matrix an Adam update's size, is J. Liu et al.'s (2025).  Matrices are row-major [rows, cols]; m = the shorter side, n = the longer one, X is [m, n].
+// 0.2 sqrt(max(rows, cols)), which gives every matrix an Adam update's size, is J. Liu et al.'s (2025).
+// Matrices are row-major [rows, cols]; m = the shorter side, n = the longer one, X is [m, n].
 //
 // Mathematics used.  With A = X X^T the iterate is X' = Q X, Q = a I + b A + c A^2, and the next Gram matrix is
 // A' = Q A Q: all of them are polynomials of one symmetric matrix, they commute, so up to three steps run on m x m
 // matrices alone, P = Q3 Q2 Q1, before X is touched again: X <- P X, A = X X^T from the new X.  Rounding errors of A grow by Q^2
 // (12 at the small end) per step on directions with tiny singular values; three steps between two true Gram matrices keep the
-// result as near to the exact one as steps on X itself, five do not (six times the error on ill-conditioned U).  Work for five
+// result of four steps and more as near to the exact one as steps on X itself, five do not (six times the error on ill-conditioned U).  Work for five
 // steps: two Gram matrices (m^2 n each, one triangle) and two products with X (2 m^2 n each) instead of five of both.
 //
 // Numerics.  Every m x n and m x m operand is held as TWO fp16 numbers, v * s = hi + lo with s a fixed power of two that keeps

@@ -13,8 +13,8 @@
 // value is still below 3e-3: less than rounding X = P U to 32 bits does.  So X is formed, and the next eight steps start from its own
 // Gram matrix.
 // v_mfma_f64_16x16x4 runs at a quarter of the rate of the fp16 pairs of muon.hip per product, but these products are small: what
-// counts is launches (3 instead of 21) and their latency.  The chain is one CU's work, 17 products of m^3 at 128 flop / cycle on one triangle's tiles with a barrier between each two: 34.7 us at m = 64,
-// 11.6 at m = 27; beyond 64 it would grow eightfold, and the four m x m buffers would not fit LDS.  A 27x64 kernel alone takes 20 us,
+// counts is launches (3 instead of 21) and their latency.  The chain is one CU's work, 17 products of m^3 at 128 flop / cycle on one
+// triangle's tiles with a barrier between each two: 34.7 us at m = 64, 11.6 at m = 27; beyond 64 it would grow eightfold, and the four m x m buffers would not fit LDS.  A 27x64 kernel alone takes 20 us,
 // eight matrices of a width-8 net 54 (gram 9, chain 35, apply 10).
 #include "muon_internal.h"
 
